@@ -435,6 +435,41 @@ int mi_softmax_backward(mi_ctx *ctx, mi_id p, mi_id dp, float scale,
 int mi_log_softmax_ce(mi_ctx *ctx, mi_id logits, mi_id targets,
                       float grad_scale, mi_id *picked, mi_id *dlogits);
 
+/* ---- log probabilities of given tokens, for answers and scores (the
+ * reference's log_softmax and pick of a target, crates/burn-tt/src/ops.rs:
+ * 5133-5166, 1001, and the greedy pick of its generation loop, crates/
+ * tt-models/src/generate.rs:176-183; no one Engine call) and for training on
+ * them.  logits [rows, cols] F32 or BF16, z = scale * logits (scale > 0, an
+ * inverse temperature), lse = ln sum exp z.  Sums and statistics are F32.  Any
+ * of the results may be left out by a null pointer:
+ *   logp [rows, 1] = z[target] - lse, with `targets` (I32, one a row; both or
+ *     neither): a target outside [0, cols) is MI_E_DOMAIN at the next wait
+ *     (logp 0);
+ *   lse [rows, 1]; entropy [rows, 1] = -sum p ln p, p = exp(z - lse);
+ *   top_logp, top_ids [rows, top] (F32, I32; both where top > 0, at most
+ *     MI_TOP_MAX and cols): the largest logits in order, mi_argmax_rows' rule
+ *     (the lowest column among equals, a NaN above every number), as
+ *     log probabilities and columns.
+ * A logit of -inf has probability 0 and adds nothing; a row of nothing but
+ * -inf gives lse and logp -inf and entropy 0.  A row with a NaN or +inf gives
+ * NaN.  All results F32. ---- */
+enum { MI_TOP_MAX = 32 };
+int mi_token_logprobs(mi_ctx *ctx, mi_id logits, mi_id targets, float scale,
+                      int64_t top, mi_id *logp, mi_id *lse, mi_id *entropy,
+                      mi_id *top_logp, mi_id *top_ids);
+/* The gradient of a loss on mi_token_logprobs' logp and entropy, from the same
+ * logits, targets and scale and the forward's lse and entropy: with g =
+ * d_logp and h = d_entropy (F32, one a row),
+ *   dlogits_j = scale * (g ([j = target] - p_j) - h p_j (z_j - lse + entropy)).
+ * d_logp (with targets) or d_entropy (with entropy) may be 0 for none, not
+ * both.  dlogits [rows, cols] F32, or BF16 rounded once.  A target out of
+ * range passes no gradient of its logp and is MI_E_DOMAIN at the next wait; a
+ * row of nothing but -inf gives zeros where no target adds its g. */
+int mi_token_logprobs_backward(mi_ctx *ctx, mi_id logits, mi_id targets,
+                               mi_id lse, mi_id entropy, mi_id d_logp,
+                               mi_id d_entropy, float scale, int out_elem,
+                               mi_id *dlogits);
+
 /* The optimizer step `param <- param - grad * lr` (burn-optim `Sgd`, no
  * momentum or decay; the reference applies it per parameter, and its traced
  * training step writes the weights in place, crates/burn-tt/src/trace.rs:
@@ -684,6 +719,50 @@ int mi_silu_mul_halves(mi_ctx *ctx, mi_id gate_up, int out_elem, mi_id *out);
 int mi_qkv_rope_cache(mi_ctx *ctx, mi_id qkv, mi_id cos_table, mi_id sin_table,
                       int64_t seq, int64_t heads, int64_t kv_heads, int64_t pos0,
                       mi_id k_cache, mi_id v_cache, int grouped, mi_id *q_out);
+/* ---- a KV cache in pages, for sequences of unequal lengths.  The reference
+ * has one slot of max_ctx rows a sequence and one position for all
+ * (crates/tt-models/src/llama.rs:403-446), no Engine counterpart.  k_pages
+ * and v_pages, both F32 or both BF16, are pools of pages:
+ * [pages * kv_heads * page, d], offset o of page p for kv head j at row
+ * (p * kv_heads + j) * page + o, `page` any number of positions.  `table`
+ * (I32 [sequences, pages a sequence]) names each sequence's pages in order,
+ * entries behind its last page unread; `lens` (I32, one a sequence) is its
+ * length, the positions of the step's new rows counted.  Both are read on
+ * the device, so a trace replays at any lengths.  A length of 0 is an idle
+ * sequence.  A cache of one slot of max_ctx rows a sequence is one of pages
+ * of max_ctx.  d in {16, 32, 64, 128}; table columns * page < 2^31. ---- */
+/* mi_qkv_rope_cache into pages: `qkv` [rows, (heads + 2 kv_heads) d] F32 or
+ * BF16 rows of the fused q|k|v projection; RoPE as mi_rope on the q and k
+ * heads at each row's own position, k and v written into the pools (BF16
+ * rounded to nearest even), q returned [rows, heads * d] as `out_elem` (F32,
+ * or BF16 rounded once).  starts 0: one row a sequence, at position
+ * lens[s] - 1 (a decode step).  Else I32 of sequences + 1 bounds, ascending
+ * from 0: rows starts[s] .. starts[s + 1] - 1 are sequence s's new positions,
+ * the last of them lens[s] - 1 (prompts one behind the other).  An idle
+ * sequence's rows and the rows behind starts[sequences] write nothing and
+ * give q rows of zeros.  A row whose position or page is out of range (the
+ * table's, the pools', the rotary tables' rows) likewise, and is MI_E_DOMAIN
+ * at the next wait.  Pages written are one sequence's alone: where two new
+ * positions name one slot, it holds either's values. */
+int mi_qkv_rope_paged(mi_ctx *ctx, mi_id qkv, mi_id cos_table, mi_id sin_table,
+                      mi_id table, mi_id lens, mi_id starts, int64_t heads,
+                      int64_t kv_heads, int64_t page, mi_id k_pages,
+                      mi_id v_pages, int out_elem, mi_id *q_out);
+/* mi_attention_rows of one new position a sequence over a cache in pages:
+ * q [sequences, heads * d] F32 or BF16, head h reading kv head
+ * h / (heads / kv_heads); row s sees positions 0 .. lens[s] - 1, its result
+ * softmax(scale q k^T) v per head with F32 sums (max clamped at -FLT_MAX, sum
+ * at FLT_MIN), out [sequences, heads * d] F32, or BF16 rounded once.  An idle
+ * sequence gives zeros.  What lies in the pools outside the sequences'
+ * positions is not looked at.  Sequences may share pages, and a table row may
+ * repeat: several new positions of one sequence are as many rows, each with
+ * its own length.  A length outside [0, table columns * page] is read as 0, a
+ * page outside the pool as page 0, and either is MI_E_DOMAIN at the next
+ * wait. */
+int mi_paged_attention(mi_ctx *ctx, mi_id q, mi_id k_pages, mi_id v_pages,
+                       mi_id table, mi_id lens, int64_t heads,
+                       int64_t kv_heads, int64_t page, float scale,
+                       int out_elem, mi_id *out);
 /* Engine::cast_float (server.rs:128): F32 <-> BF16, ties to even, NaN kept
  * a NaN; and I32 -> F32 (`as f32`).  `out_elem` MI_BF16_PARTS: an F32
  * buffer's parts (columns a multiple of 4). */

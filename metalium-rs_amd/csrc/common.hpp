@@ -357,6 +357,21 @@ int refuse_if_capturing(Ctx *ctx, const char *what);
 // Kernel-side flag word for the context.
 inline uint32_t *flags(Ctx *ctx) { return ctx->dev_flags; }
 
+// The context's device current for the length of a call (an allocation and a
+// launch go to the current device), the caller's restored behind it.
+struct DeviceGuard {
+  int was = -1;
+  explicit DeviceGuard(const Ctx *ctx) {
+    if (hipGetDevice(&was) != hipSuccess || was == ctx->device) was = -1;
+    else (void)hipSetDevice(ctx->device);
+  }
+  ~DeviceGuard() {
+    if (was >= 0) (void)hipSetDevice(was);
+  }
+  DeviceGuard(const DeviceGuard &) = delete;
+  DeviceGuard &operator=(const DeviceGuard &) = delete;
+};
+
 // Grid sizing: blocks to cover `n` items at `per_block`, capped.
 inline unsigned grid_for(int64_t n, int64_t per_block, int64_t cap = 1 << 20) {
   int64_t g = (n + per_block - 1) / per_block;

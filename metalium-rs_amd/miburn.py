@@ -18,7 +18,7 @@ from __future__ import annotations
 import ctypes
 import weakref
 import os
-from typing import Optional, Sequence, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import numpy as np
 
@@ -69,6 +69,15 @@ class MiError(RuntimeError):
         super().__init__(f"{self.kind}: {msg}")
 
 
+class TokenLogprobs(NamedTuple):
+    """Engine.token_logprobs' result ids; 0 where one was not asked for."""
+    logp: int
+    lse: int
+    entropy: int
+    top_logp: int
+    top_ids: int
+
+
 class Report(ctypes.Structure):
     _fields_ = [(n, ctypes.c_uint64) for n in (
         "ops", "uploads", "downloads", "bytes_up", "bytes_down", "live_buffers", "device_bytes",
@@ -117,6 +126,10 @@ def _load() -> ctypes.CDLL:
         "mi_attention_rows": [P, U64, U64, U64, I64, I64, I64, I64, I64, c_float, Ip],
         "mi_attention_rows_as": [P, U64, U64, U64, I64, I64, I64, I64, I64, c_float, c_int, Ip],
         "mi_attention_rows_into": [P, U64, U64, U64, I64, I64, I64, I64, I64, c_float, U64],
+        "mi_qkv_rope_paged": [P, U64, U64, U64, U64, U64, U64, I64, I64, I64, U64, U64, c_int, Ip],
+        "mi_paged_attention": [P, U64, U64, U64, U64, U64, I64, I64, I64, c_float, c_int, Ip],
+        "mi_token_logprobs": [P, U64, U64, c_float, I64, Ip, Ip, Ip, Ip, Ip],
+        "mi_token_logprobs_backward": [P, U64, U64, U64, U64, U64, U64, c_float, c_int, Ip],
         "mi_reduce_then": [P, U64, c_int, c_int, c_u32, c_float, Ip],
         "mi_add_rms_norm": [P, U64, U64, U64, c_float, Ip, Ip],
         "mi_matmul_pairs": [P, U64, U64, I64, ctypes.POINTER(I64), ctypes.POINTER(c_int), ctypes.POINTER(I64),
@@ -345,6 +358,22 @@ class Engine:
         self._check(self._lib.mi_log_softmax_ce(self.ctx, logits, targets, grad_scale, ctypes.byref(a), ctypes.byref(b)))
         return a.value, b.value
 
+    def token_logprobs(self, logits: int, targets: int = 0, scale: float = 1.0, top: int = 0) -> TokenLogprobs:
+        """Each row's log probability of its target (targets 0: none), log sum,
+        entropy and `top` likeliest columns, of softmax(scale * logits)."""
+        ids = [ctypes.c_uint64() for _ in range(5)]
+        want = (bool(targets), True, True, top > 0, top > 0)
+        self._check(self._lib.mi_token_logprobs(self.ctx, logits, targets, scale, top,
+                                                *[ctypes.byref(i) if w else None for i, w in zip(ids, want)]))
+        return TokenLogprobs(*[i.value for i in ids])
+
+    def token_logprobs_backward(self, logits: int, targets: int, lse: int, entropy: int, d_logp: int, d_entropy: int,
+                                scale: float = 1.0, out_elem: int = F32) -> int:
+        """dlogits from the gradients of token_logprobs' logp and entropy
+        (targets and d_logp, or entropy and d_entropy, 0 for none)."""
+        return self._out(self._lib.mi_token_logprobs_backward, logits, targets, lse, entropy, d_logp, d_entropy, scale,
+                         out_elem)
+
     def matmul_items(self, a: int, a_t: bool, a_at, b: int, b_t: bool, b_at, groups: int, per_group: int, m: int,
                      k: int, n: int, out: int, out_at) -> None:
         """Grouped strided products written in place into `out`; each `*_at`
@@ -393,6 +422,20 @@ class Engine:
         """Prefill q|k|v tail: RoPE on q and k, k and v into the caches; returns q."""
         return self._out(self._lib.mi_qkv_rope_cache, qkv, cos, sin, seq, heads, kv_heads, pos0, k_cache, v_cache,
                          int(grouped))
+
+    def qkv_rope_paged(self, qkv: int, cos: int, sin: int, table: int, lens: int, starts: int, heads: int,
+                       kv_heads: int, page: int, k_pages: int, v_pages: int, out_elem: int = F32) -> int:
+        """qkv_rope_cache into a paged cache, each row at its own sequence's
+        position (starts 0: one row a sequence); returns q [rows, heads * d]."""
+        return self._out(self._lib.mi_qkv_rope_paged, qkv, cos, sin, table, lens, starts, heads, kv_heads, page,
+                         k_pages, v_pages, out_elem)
+
+    def paged_attention(self, q: int, k_pages: int, v_pages: int, table: int, lens: int, heads: int, kv_heads: int,
+                        page: int, scale: float, out_elem: int = F32) -> int:
+        """Attention of one new position a sequence over the first lens[s]
+        positions its row of the page table names."""
+        return self._out(self._lib.mi_paged_attention, q, k_pages, v_pages, table, lens, heads, kv_heads, page, scale,
+                         out_elem)
 
     def norm_qkv_rope(self, x: int, gamma: int, eps: float, w_qkv: int, cos: int, sin: int, heads: int,
                       kv_heads: int, pos: int, k_cache: int, v_cache: int) -> int:

@@ -1,0 +1,15 @@
+// The paged cache's index arithmetic (metalium-rs_amd/csrc/paged.hpp) as a
+// host library for test_paged_index.py.
+#include "../metalium-rs_amd/csrc/paged.hpp"
+
+extern "C" {
+int pos_of(int64_t r, int64_t first, int64_t end, int64_t len, int64_t cap, int64_t *pos) {
+  const mi::PagedPos p = mi::paged_pos(r, first, end, len, cap);
+  *pos = p.pos;
+  return p.state;
+}
+int64_t row_of(int64_t p, int64_t j, int64_t o, int64_t kv_heads, int64_t page) {
+  return mi::paged_row(p, j, o, kv_heads, page);
+}
+int64_t len_of(int64_t len, int64_t cap) { return mi::paged_len(len, cap); }
+}
