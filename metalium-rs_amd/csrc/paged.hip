@@ -50,6 +50,8 @@ int paged_cache(Ctx *ctx, const char *what, mi_id k_pages, mi_id v_pages, mi_id 
     return fail(ctx, MI_E_ARG, "%s: table %s [%lld, %lld] and lengths %s [%lld, %lld], want I32 [sequences, pages] and I32 of one a sequence",
                 what, elem_name(tb->elem), (long long)tb->rows, (long long)tb->cols, elem_name(lb->elem),
                 (long long)lb->rows, (long long)lb->cols);
+  if (kb->rows > INT32_MAX)
+    return fail(ctx, MI_E_UNSUPPORTED, "%s: pools of %lld rows (at most 2^31 - 1)", what, (long long)kb->rows);
   if (tb->cols > INT32_MAX / page)
     return fail(ctx, MI_E_UNSUPPORTED, "%s: a table row of %lld pages of %lld positions (at most 2^31 - 1)", what,
                 (long long)tb->cols, (long long)page);
@@ -160,89 +162,566 @@ void append_launch(Ctx *ctx, const AppendArgs &a, int64_t D, int out_elem) {
 }
 
 // --------------------------------------------------------------- attention
+// One new token a sequence: softmax(scale q K^T) V over the sequence's pages.
+// Every byte of K and V is read once for a kv head's G query heads, so the
+// operator is bound by HBM; the products are small (4 G D operations a
+// position) and run on the matrix cores, which read their operands as the
+// cache holds them:
+//   S^T = K Q^T, 16 positions x 16 heads: a lane's 16 bytes of a key row are
+//     its operand (a row of K = D contraction steps);
+//   O^T = V^T P^T, 16 columns x 16 heads: P^T is S^T's own result layout (lane
+//     (head h, group g) holds positions 4 g .. 4 g + 3 of head h), and V^T's
+//     operand, four positions of one column, is a 4 x 4 transpose within the
+//     lane's own registers.
+// So nothing passes through LDS between the two products.  BF16 pools: the
+// F32 queries (scaled, in base 2) and the weights go as three BF16 parts each
+// (24 bits, small parts first), K and V as they are -- F32 sums of exact
+// products.  F32 pools: the F32 matrix cores.
+//
+// The sequences are cut into chunks of nearly equal length (paged.hpp), a
+// block each: lengths are known on the device only, so every wavefront forms
+// the cut from them itself, and the grid is its upper bound.  A block's four
+// wavefronts take steps of POS positions in turn, each with running maximum
+// and sum, and join in LDS; a chunk of a cut sequence leaves its maximum, sum
+// and sums of values to a second launch that joins them.
+
+typedef __bf16 pa_bf16x8 __attribute__((ext_vector_type(8)));
+typedef float pa_f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int PA_WAVES = 4;
+constexpr int PA_HEADS = 16;       // query heads a block: the matrix cores' tile
+constexpr int PA_UNIT = 64;        // chunk lengths are multiples of it
+constexpr int64_t PA_BLOCKS = 1024;  // blocks the lengths are cut for
+
+// Positions a wavefront takes a step: 8 KiB of keys.
+template <int D, typename TC>
+constexpr int pa_pos() { return 8192 / (D * static_cast<int>(sizeof(TC))) > 64 ? 64 : 8192 / (D * static_cast<int>(sizeof(TC))); }
 
 struct AttendArgs {
   const void *q, *k, *v;
   const int32_t *table, *lens;
   int64_t seqs, per, pages, page;
-  int heads, kv_heads;
-  float scale;
+  PageDiv div;
+  int heads, kv_heads, group, tiles, live;  // heads a kv head, their tiles of 16, heads a tile at most
+  int q16, out16;
+  int64_t target;  // chunks the lengths are cut for
+  int64_t slots;   // partials there is room for, a kv head tile
+  float scale;     // times log2(e)
+  float *part;
   void *out;
   uint32_t *flags;
 };
 
-// One wavefront a (sequence, query head), 64 positions a step: a lane forms
-// the score of its position, the running maximum and sum rescale what was
-// gathered, and the value rows are added with a lane a column.
-template <int D, typename TQ, typename TC, typename TO>
-__global__ void __launch_bounds__(64) attend_kernel(AttendArgs a) {
-  __shared__ float qs[D];
-  const int64_t s = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
-  const int lane = threadIdx.x;
-  const int64_t j = h / (a.heads / a.kv_heads), cap = a.per * a.page;
-  const TQ *q = static_cast<const TQ *>(a.q) + (s * a.heads + h) * D;
-  for (int c = 4 * lane; c < D; c += 256) *reinterpret_cast<float4 *>(qs + c) = f32x4_get(q + c);
-  __syncthreads();
-  const int64_t raw = a.lens[s], len = paged_len(raw, cap);
-  if (raw != len && lane == 0) atomicOr(a.flags, FLAG_INDEX_RANGE);
-  const TC *K = static_cast<const TC *>(a.k), *V = static_cast<const TC *>(a.v);
-  constexpr int CPL = (D + 63) / 64;
-  float m = -FLT_MAX, l = 0.0f, acc[CPL] = {};
-  for (int64_t p0 = 0; p0 < len; p0 += 64) {
-    const int64_t p = p0 + lane < len ? p0 + lane : len - 1;
-    int64_t pg = a.table[s * a.per + p / a.page];
-    if (pg < 0 || pg >= a.pages) {
-      atomicOr(a.flags, FLAG_INDEX_RANGE);
-      pg = 0;
+// Floats of one chunk's partial: `live` maxima, `live` sums, zeros to a
+// multiple of 4, then each head's D sums.
+__host__ __device__ constexpr int64_t pa_acc0(int64_t live) { return (2 * live + 3) / 4 * 4; }
+__host__ __device__ constexpr int64_t pa_stride(int64_t live, int64_t D) { return pa_acc0(live) + live * D; }
+
+// Inclusive sums over the wavefront's lanes.
+__device__ __forceinline__ int32_t wave_scan(int32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+__device__ __forceinline__ int32_t lane_value(int32_t v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+
+// The lengths of 64 sequences from s0, a lane each (0 past the last), and
+// their sum over all sequences.
+__device__ __forceinline__ int32_t pa_len(const AttendArgs &a, int64_t s0, int lane) {
+  if (s0 + lane >= a.seqs) return 0;
+  return static_cast<int32_t>(paged_len(a.lens[s0 + lane], a.per * a.page));
+}
+__device__ __forceinline__ int64_t pa_sum(const AttendArgs &a, int lane, int32_t first) {
+  int64_t t = first;
+#pragma unroll 4
+  for (int64_t s0 = 64; s0 < a.seqs; s0 += 64) t += pa_len(a, s0, lane);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) t += __shfl_xor(t, o, 64);
+  return t;
+}
+
+// A chunk of the cut: its sequence (-1 past the last chunk), its number of n,
+// the sequence's length, and the slot of the sequence's first partial.
+struct Chunk {
+  int64_t seq;
+  int32_t c, n, len, slot;
+};
+// Chunk g; or (by_seq) the cut of sequence g.
+template <bool BY_SEQ>
+__device__ __forceinline__ Chunk pa_chunk(const AttendArgs &a, int64_t g, int lane) {
+  int32_t len = pa_len(a, 0, lane);
+  const int64_t limit = chunk_limit(pa_sum(a, lane, len), a.target, PA_UNIT);
+  int64_t before = 0, slot = 0;
+  for (int64_t s0 = 0; s0 < a.seqs; s0 += 64) {
+    if (s0) len = pa_len(a, s0, lane);
+    const int32_t n = s0 + lane < a.seqs ? chunk_count(len, limit) : 0, cut = n > 1 ? n : 0;
+    const int32_t in = wave_scan(n), cuts = wave_scan(cut);
+    const int64_t all = lane_value(in, 63);
+    int at = -1;
+    if constexpr (BY_SEQ) {
+      if (g < s0 + 64) at = static_cast<int>(g - s0);
+    } else {
+      if (g < before + all) at = __popcll(__ballot(before + in <= g));
     }
-    const int64_t row = paged_row(pg, j, p % a.page, a.kv_heads, a.page);
-    float sc = 0.0f;
-    for (int c = 0; c < D; c += 4) {
-      const float4 kv = f32x4_get(K + row * D + c), qv = *reinterpret_cast<const float4 *>(qs + c);
-      sc += (qv.x * kv.x + qv.y * kv.y) + (qv.z * kv.z + qv.w * kv.w);
+    if (at >= 0) {
+      at = __builtin_amdgcn_readfirstlane(at);
+      const int32_t mine = lane_value(n, at);
+      Chunk r;
+      r.seq = s0 + at;
+      r.n = mine;
+      r.c = static_cast<int32_t>(g - before) - (lane_value(in, at) - mine);
+      r.len = lane_value(len, at);
+      r.slot = static_cast<int32_t>(slot) + lane_value(cuts, at) - (mine > 1 ? mine : 0);
+      return r;
     }
-    sc = p0 + lane < len ? sc * a.scale : -INFINITY;
-    const float mn = max_nan(m, fold_max<64>(sc));
-    const float w = expf(m - mn), e = p0 + lane < len ? expf(sc - mn) : 0.0f;
-    l = l * w + fold_sum<64>(e);
-    m = mn;
-    for (int i = 0; i < CPL; ++i) acc[i] *= w;
-    const int n = static_cast<int>(len - p0 < 64 ? len - p0 : 64);
-    for (int t = 0; t < n; ++t) {
-      const float pt = __shfl(e, t, 64);
-      const int64_t rt = __shfl(row, t, 64);
-      for (int i = 0; i < CPL; ++i) {
-        const int c = i * 64 + lane;
-        if (c < D) {
-          float x;
-          if constexpr (sizeof(TC) == 2) x = bf16_bits_to_f32(V[rt * D + c]);
-          else x = V[rt * D + c];
-          acc[i] += pt * x;
+    before += all;
+    slot += lane_value(cuts, 63);
+  }
+  return Chunk{-1, 0, 0, 0, 0};
+}
+
+// Three BF16 parts of two F32 values, packed (a in the low halves): each the
+// rounding of what the ones before leave.
+__device__ __forceinline__ void split3(float a, float b, uint32_t &h, uint32_t &m, uint32_t &l) {
+  h = bf16x2_bits(a, b);
+  a -= __uint_as_float(h << 16);
+  b -= __uint_as_float(h & 0xffff0000u);
+  m = bf16x2_bits(a, b);
+  l = bf16x2_bits(a - __uint_as_float(m << 16), b - __uint_as_float(m & 0xffff0000u));
+}
+
+__device__ __forceinline__ pa_f32x4 pa_mfma(uint4 a, uint4 b, pa_f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pa_bf16x8, a), __builtin_bit_cast(pa_bf16x8, b), c,
+                                                 0, 0, 0);
+}
+
+// The maximum over the four lanes of one head (l, l ^ 16, l ^ 32, l ^ 48).
+__device__ __forceinline__ float head_max(float v) {
+  float x, y;
+  swap16_pair(v, x, y);
+  v = max_nan(x, y);
+  swap32_pair(v, x, y);
+  return max_nan(x, y);
+}
+
+// One wavefront's part of a chunk on BF16 pools.
+template <int D>
+struct WaveBf16 {
+  static constexpr int POS = pa_pos<D, uint16_t>();
+  static constexpr int NT = POS / 16, KS = D < 32 ? 1 : D / 32, CP = D / 16;  // key steps; columns a lane
+  uint4 q[3][KS];
+  uint4 k[NT][KS];
+  uint32_t v[NT][4][CP < 2 ? 1 : CP / 2];
+  pa_f32x4 acc[CP];
+
+  __device__ __forceinline__ void query(const float *qs, int lane) {  // LDS [16][D + 4]
+    const int h = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < KS; ++t) {
+      uint32_t w[3][4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int c = 32 * t + 8 * g + 2 * e;
+        const float2 x = c < D ? *reinterpret_cast<const float2 *>(qs + h * (D + 4) + c) : make_float2(0.f, 0.f);
+        split3(x.x, x.y, w[0][e], w[1][e], w[2][e]);
+      }
+#pragma unroll
+      for (int p = 0; p < 3; ++p) q[p][t] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+    }
+  }
+  __device__ __forceinline__ void load_k(const uint16_t *K, const int32_t *rows, int lane) {
+    const int g = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const uint16_t *p = K + static_cast<int64_t>(rows[16 * t + (lane & 15)]) * D + (D < 32 ? 8 * (g & 1) : 8 * g);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) k[t][s] = *reinterpret_cast<const uint4 *>(p + 32 * s);
+    }
+  }
+  __device__ __forceinline__ void load_v(const uint16_t *V, const int32_t *rows, int lane) {
+    const int n = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int4 r4 = *reinterpret_cast<const int4 *>(rows + 16 * t + 4 * g);
+      const int32_t r[4] = {r4.x, r4.y, r4.z, r4.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint16_t *p = V + static_cast<int64_t>(r[j]) * D + CP * n;
+        if constexpr (CP == 8) {
+          const uint4 x = *reinterpret_cast<const uint4 *>(p);
+          v[t][j][0] = x.x; v[t][j][1] = x.y; v[t][j][2] = x.z; v[t][j][3] = x.w;
+        } else if constexpr (CP == 4) {
+          const uint2 x = *reinterpret_cast<const uint2 *>(p);
+          v[t][j][0] = x.x; v[t][j][1] = x.y;
+        } else if constexpr (CP == 2) {
+          v[t][j][0] = *reinterpret_cast<const uint32_t *>(p);
+        } else {
+          v[t][j][0] = *p;
         }
       }
     }
   }
-  const float den = isnan(l) ? l : (l > FLT_MIN ? l : FLT_MIN);
-  TO *o = static_cast<TO *>(a.out) + (s * a.heads + h) * D;
-  for (int i = 0; i < CPL; ++i)
-    if (i * 64 + lane < D) f32_put(o + i * 64 + lane, acc[i] / den);
+  // Scores of tile t, positions 4 g + i of head lane & 15.  D = 16: the
+  // upper half of the contraction meets zeros of q.
+  __device__ __forceinline__ pa_f32x4 scores(int t) const {
+    pa_f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int p = 2; p >= 0; --p)
+#pragma unroll
+      for (int u = 0; u < KS; ++u) s = pa_mfma(k[t][u], q[p][u], s);
+    return s;
+  }
+  // acc += V^T P^T over all tiles, two at a time: contraction step 8 g + j is
+  // position 4 g + j % 4 of tile j / 4 of the pair, for both operands.
+  __device__ __forceinline__ void values(const pa_f32x4 (&p)[NT]) {
+    static_assert(NT % 2 == 0, "tiles in pairs");
+#pragma unroll
+    for (int t = 0; t < NT; t += 2) {
+      uint32_t w[3][4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        split3(p[t + e / 2][2 * (e & 1)], p[t + e / 2][2 * (e & 1) + 1], w[0][e], w[1][e], w[2][e]);
+#pragma unroll
+      for (int c = 0; c < CP; ++c) {
+        const uint32_t sel = c & 1 ? 0x07060302u : 0x05040100u;
+        const int d = c >> 1;
+        const uint4 x = make_uint4(__builtin_amdgcn_perm(v[t][1][d], v[t][0][d], sel),
+                                   __builtin_amdgcn_perm(v[t][3][d], v[t][2][d], sel),
+                                   __builtin_amdgcn_perm(v[t + 1][1][d], v[t + 1][0][d], sel),
+                                   __builtin_amdgcn_perm(v[t + 1][3][d], v[t + 1][2][d], sel));
+#pragma unroll
+        for (int q_ = 2; q_ >= 0; --q_) acc[c] = pa_mfma(x, make_uint4(w[q_][0], w[q_][1], w[q_][2], w[q_][3]), acc[c]);
+      }
+    }
+  }
+};
+
+// The same on F32 pools: 16 x 16 x 4 steps of the F32 matrix cores, whose
+// operand is one value a lane (row or column lane & 15, step lane >> 4).
+template <int D>
+struct WaveF32 {
+  static constexpr int POS = pa_pos<D, float>();
+  static constexpr int NT = POS / 16, KQ = D / 16, CP = D / 16;
+  float4 q[KQ];
+  float4 k[NT][KQ];
+  float v[NT][4][CP];
+  pa_f32x4 acc[CP];
+
+  __device__ __forceinline__ void query(const float *qs, int lane) {
+#pragma unroll
+    for (int u = 0; u < KQ; ++u) q[u] = *reinterpret_cast<const float4 *>(qs + (lane & 15) * (D + 4) + 16 * u + 4 * (lane >> 4));
+  }
+  __device__ __forceinline__ void load_k(const float *K, const int32_t *rows, int lane) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const float *p = K + static_cast<int64_t>(rows[16 * t + (lane & 15)]) * D + 4 * (lane >> 4);
+#pragma unroll
+      for (int u = 0; u < KQ; ++u) k[t][u] = *reinterpret_cast<const float4 *>(p + 16 * u);
+    }
+  }
+  __device__ __forceinline__ void load_v(const float *V, const int32_t *rows, int lane) {
+    const int n = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int4 r4 = *reinterpret_cast<const int4 *>(rows + 16 * t + 4 * g);
+      const int32_t r[4] = {r4.x, r4.y, r4.z, r4.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float *p = V + static_cast<int64_t>(r[j]) * D + CP * n;
+        if constexpr (CP >= 4) {
+#pragma unroll
+          for (int c = 0; c < CP; c += 4) {
+            const float4 x = *reinterpret_cast<const float4 *>(p + c);
+            v[t][j][c] = x.x; v[t][j][c + 1] = x.y; v[t][j][c + 2] = x.z; v[t][j][c + 3] = x.w;
+          }
+        } else if constexpr (CP == 2) {
+          const float2 x = *reinterpret_cast<const float2 *>(p);
+          v[t][j][0] = x.x; v[t][j][1] = x.y;
+        } else {
+          v[t][j][0] = *p;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ pa_f32x4 scores(int t) const {
+    pa_f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < KQ; ++u) {
+      s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][u].x, q[u].x, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][u].y, q[u].y, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][u].z, q[u].z, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][u].w, q[u].w, s, 0, 0, 0);
+    }
+    return s;
+  }
+  __device__ __forceinline__ void values(const pa_f32x4 (&p)[NT]) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int c = 0; c < CP; ++c) acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[t][j][c], p[t][j], acc[c], 0, 0, 0);
+  }
+};
+
+template <int D, typename TC>
+struct WaveOf { using type = WaveF32<D>; };
+template <int D>
+struct WaveOf<D, uint16_t> { using type = WaveBf16<D>; };
+
+template <int D, typename TC>
+__global__ void __launch_bounds__(PA_WAVES * 64) attend_kernel(AttendArgs a) {
+  using W = typename WaveOf<D, TC>::type;
+  constexpr int POS = W::POS, NT = W::NT, CP = W::CP, QS = D + 4;
+  // The scaled queries, then (once read) the wavefronts' results.
+  __shared__ float sm[PA_WAVES * PA_HEADS * QS];
+  __shared__ float stat[PA_WAVES][2][PA_HEADS];
+  __shared__ __align__(16) int32_t rowbuf[PA_WAVES][2][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int parts = a.kv_heads * a.tiles;
+  const int64_t g = blockIdx.x / parts;
+  const int jt = blockIdx.x % parts, j = jt / a.tiles, h0 = (jt % a.tiles) * PA_HEADS;
+  const Chunk ch = pa_chunk<false>(a, g, lane);
+  if (ch.seq < 0) return;
+  const int nh = a.group - h0 < PA_HEADS ? a.group - h0 : PA_HEADS;  // heads of this tile
+  const int32_t clen = chunk_len(ch.len, ch.n, PA_UNIT);
+  const int64_t from = static_cast<int64_t>(ch.c) * clen;
+  const int32_t lo = from < ch.len ? static_cast<int32_t>(from) : ch.len;
+  const int32_t hi = ch.len - lo < clen ? ch.len : lo + clen;
+  if (tid == 0 && ch.c == 0 && a.lens[ch.seq] != ch.len) atomicOr(a.flags, FLAG_INDEX_RANGE);
+
+  // Queries, scaled, heads past the tile's as zeros.
+  const int64_t q0 = (ch.seq * a.heads + static_cast<int64_t>(j) * a.group + h0) * D;
+  for (int e = 4 * tid; e < PA_HEADS * D; e += 4 * PA_WAVES * 64) {
+    const int h = e / D, c = e % D;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (h < nh) x = a.q16 ? f32x4_get(static_cast<const uint16_t *>(a.q) + q0 + e) : f32x4_get(static_cast<const float *>(a.q) + q0 + e);
+    *reinterpret_cast<float4 *>(sm + h * QS + c) = make_float4(x.x * a.scale, x.y * a.scale, x.z * a.scale, x.w * a.scale);
+  }
+  __syncthreads();
+
+  W w;
+  w.query(sm, lane);
+#pragma unroll
+  for (int c = 0; c < CP; ++c) w.acc[c] = pa_f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -FLT_MAX, l = 0.0f;
+  const TC *K = static_cast<const TC *>(a.k), *V = static_cast<const TC *>(a.v);
+  const int32_t *trow = a.table + ch.seq * a.per;
+  const int32_t stride = static_cast<int32_t>(a.kv_heads * a.page), jrow = static_cast<int32_t>(j * a.page);
+  const int32_t steps = (hi - lo + POS - 1) / POS;
+  int32_t (*rows)[64] = rowbuf[wave];
+  // The pool rows of a step's positions, those past the chunk's end the
+  // last one's again (their scores are dropped below): page ids a step
+  // ahead, so their latency is off the loop.
+  auto position = [&](int32_t i) {
+    const int32_t p = lo + i * POS + (lane & (POS - 1));
+    return p < hi ? p : hi - 1;
+  };
+  auto page_id = [&](int32_t i) { return trow[page_of(static_cast<uint32_t>(position(i)), a.div)]; };
+  auto put_rows = [&](int32_t i, int32_t id, int b) {
+    const int32_t p = position(i);
+    if (id < 0 || id >= a.pages) {
+      atomicOr(a.flags, FLAG_INDEX_RANGE);
+      id = 0;
+    }
+    if (lane < POS)
+      rows[b][lane] = id * stride + jrow + (p - static_cast<int32_t>(page_of(static_cast<uint32_t>(p), a.div) * a.page));
+    __builtin_amdgcn_wave_barrier();  // read below by this wavefront, whose LDS accesses run in order
+  };
+  int32_t i = wave, id = 0;
+  int b = 0;
+  if (i < steps) {
+    put_rows(i, page_id(i), 0);
+    if (i + PA_WAVES < steps) id = page_id(i + PA_WAVES);
+    w.load_k(K, rows[0], lane);
+  }
+  for (; i < steps; i += PA_WAVES, b ^= 1) {
+    w.load_v(V, rows[b], lane);
+    const bool more = i + PA_WAVES < steps;
+    if (more) {
+      put_rows(i + PA_WAVES, id, b ^ 1);
+      if (i + 2 * PA_WAVES < steps) id = page_id(i + 2 * PA_WAVES);
+    }
+    pa_f32x4 s[NT];
+    float mx = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) s[t] = w.scores(t);
+    if (more) w.load_k(K, rows[b ^ 1], lane);
+    const int32_t left = hi - lo - i * POS;  // positions from this step's first
+    if (left < POS) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (16 * t + 4 * (lane >> 4) + e >= left) s[t][e] = -INFINITY;
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx = max_nan(mx, s[t][e]);
+    const float mn = max_nan(m, head_max(mx));
+    const float r = __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    l *= r;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[t][e] = __builtin_amdgcn_exp2f(s[t][e] - mn);
+        l += s[t][e];
+      }
+#pragma unroll
+    for (int c = 0; c < CP; ++c) w.acc[c] *= r;
+    w.values(s);
+  }
+  l = fold_columns<16>(l);
+
+  // The wavefronts' results through LDS: head h's D sums at [wave][h][QS].
+  __syncthreads();
+  {
+    const int h = lane & 15, gq = lane >> 4;
+    if (lane < PA_HEADS) {
+      stat[wave][0][lane] = m;
+      stat[wave][1][lane] = l;
+    }
+    float *dst = sm + (wave * PA_HEADS + h) * QS;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int c = 0; c < CP; ++c) dst[CP * (4 * gq + e) + c] = w.acc[c][e];
+  }
+  __syncthreads();
+  float *part = nullptr;
+  if (ch.n > 1) {
+    const int64_t slot = ch.slot + ch.c;
+    if (slot >= a.slots) return;  // never: the cut's bound
+    part = a.part + (slot * parts + jt) * pa_stride(a.live, D);
+  }
+  for (int e = tid; e < nh * D; e += PA_WAVES * 64) {
+    const int h = e / D, c = e % D;
+    float M = stat[0][0][h];
+#pragma unroll
+    for (int x = 1; x < PA_WAVES; ++x) M = max_nan(M, stat[x][0][h]);
+    float sum = 0.0f, den = 0.0f;
+#pragma unroll
+    for (int x = 0; x < PA_WAVES; ++x) {
+      const float wt = __builtin_amdgcn_exp2f(stat[x][0][h] - M);
+      den += wt * stat[x][1][h];
+      sum += wt * sm[(x * PA_HEADS + h) * QS + c];
+    }
+    if (part) {
+      if (c == 0) {
+        part[h] = M;
+        part[a.live + h] = den;
+      }
+      part[pa_acc0(a.live) + e] = sum;
+    } else {
+      den = isnan(den) ? den : (den > FLT_MIN ? den : FLT_MIN);
+      if (a.out16) f32_put(static_cast<uint16_t *>(a.out) + q0 + e, sum / den);
+      else static_cast<float *>(a.out)[q0 + e] = sum / den;
+    }
+  }
 }
 
-template <int D, typename TQ, typename TC>
-void attend_launch(Ctx *ctx, const AttendArgs &a, int out_elem) {
-  const unsigned grid = static_cast<unsigned>(a.seqs * a.heads);
-  if (out_elem == MI_BF16) attend_kernel<D, TQ, TC, uint16_t><<<grid, 64, 0, ctx->stream>>>(a);
-  else attend_kernel<D, TQ, TC, float><<<grid, 64, 0, ctx->stream>>>(a);
-}
+// Joins the chunks of a cut sequence, a block a (sequence, query head): the
+// chunks' weights 2^(m_c - M) in LDS, then D / 4 lanes a group, the groups
+// taking the chunks in turn, and the groups' sums added in order.
 template <int D>
-void attend_types(Ctx *ctx, const AttendArgs &a, int q_elem, int cache_elem, int out_elem) {
-  if (q_elem == MI_BF16) {
-    if (cache_elem == MI_BF16) attend_launch<D, uint16_t, uint16_t>(ctx, a, out_elem);
-    else attend_launch<D, uint16_t, float>(ctx, a, out_elem);
-  } else {
-    if (cache_elem == MI_BF16) attend_launch<D, float, uint16_t>(ctx, a, out_elem);
-    else attend_launch<D, float, float>(ctx, a, out_elem);
+__global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a) {
+  constexpr int LP = D / 4, NG = 256 / LP;
+  extern __shared__ float wts[];  // a chunk each
+  __shared__ float red[4];
+  __shared__ float4 sums[256];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t s = blockIdx.x / a.heads;
+  const int h = static_cast<int>(blockIdx.x % a.heads);
+  const Chunk ch = pa_chunk<true>(a, s, lane);
+  if (ch.n < 2 || ch.slot + ch.n > a.slots) return;
+  const int j = h / a.group, hg = h % a.group, jt = j * a.tiles + hg / PA_HEADS, ht = hg % PA_HEADS;
+  const int64_t parts = a.kv_heads * a.tiles, ps = pa_stride(a.live, D);
+  const float *p = a.part + (static_cast<int64_t>(ch.slot) * parts + jt) * ps;
+  const int64_t step = parts * ps;
+  float M = -INFINITY;
+  for (int c = tid; c < ch.n; c += 256) {
+    const float mc = p[c * step + ht];
+    wts[c] = mc;
+    M = max_nan(M, mc);
   }
+  M = fold_max<64>(M);
+  if (lane == 0) red[wave] = M;
+  __syncthreads();
+  M = max_nan(max_nan(red[0], red[1]), max_nan(red[2], red[3]));
+  __syncthreads();
+  float den = 0.0f;
+  for (int c = tid; c < ch.n; c += 256) {
+    const float wt = __builtin_amdgcn_exp2f(wts[c] - M);
+    wts[c] = wt;
+    den += wt * p[c * step + a.live + ht];
+  }
+  den = fold_sum<64>(den);
+  if (lane == 0) red[wave] = den;
+  __syncthreads();
+  den = (red[0] + red[1]) + (red[2] + red[3]);
+  den = isnan(den) ? den : (den > FLT_MIN ? den : FLT_MIN);
+  const int grp = tid / LP, c4 = 4 * (tid % LP);
+  const float *pv = p + pa_acc0(a.live) + ht * D + c4;
+  float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int c = grp; c < ch.n; c += NG) {
+    const float4 x = *reinterpret_cast<const float4 *>(pv + c * step);
+    const float wt = wts[c];
+    t.x += wt * x.x;
+    t.y += wt * x.y;
+    t.z += wt * x.z;
+    t.w += wt * x.w;
+  }
+  sums[tid] = t;
+  __syncthreads();
+  if (tid < LP) {
+    t = sums[tid];
+#pragma unroll
+    for (int x = 1; x < NG; ++x) {
+      const float4 o = sums[x * LP + tid];
+      t.x += o.x;
+      t.y += o.y;
+      t.z += o.z;
+      t.w += o.w;
+    }
+    t = make_float4(t.x / den, t.y / den, t.z / den, t.w / den);
+    const int64_t at = (s * a.heads + h) * D + 4 * tid;
+    if (a.out16) f32x4_put(static_cast<uint16_t *>(a.out) + at, t);
+    else f32x4_put(static_cast<float *>(a.out) + at, t);
+  }
+}
+
+template <int D>
+int attend_launch(Ctx *ctx, AttendArgs a, bool kv16) {
+  const int64_t parts = static_cast<int64_t>(a.kv_heads) * a.tiles, cap = a.per * a.page;
+  a.target = PA_BLOCKS / parts > 1 ? PA_BLOCKS / parts : 1;
+  // A sequence makes one chunk and at most one more a unit; all of them
+  // together at most the target's beside one each.
+  const int64_t most = (cap + PA_UNIT - 1) / PA_UNIT;
+  int64_t chunks = a.target + 1 + a.seqs;
+  if (most < chunks / a.seqs) chunks = (most > 1 ? most : 1) * a.seqs;
+  const bool cut = most > 1;
+  a.slots = cut ? 2 * a.target + 2 : 0;
+  if (chunks * parts > INT32_MAX || a.seqs * a.heads > INT32_MAX)
+    return fail(ctx, MI_E_UNSUPPORTED, "paged_attention: grid too large");
+  if (cut) {
+    a.part = static_cast<float *>(scratch(ctx, static_cast<size_t>(a.slots * parts * pa_stride(a.live, D)) * sizeof(float)));
+    if (!a.part) return fail(ctx, MI_E_OOM, "paged_attention scratch");
+  }
+  const unsigned grid = static_cast<unsigned>(chunks * parts);
+  if (kv16) attend_kernel<D, uint16_t><<<grid, PA_WAVES * 64, 0, ctx->stream>>>(a);
+  else attend_kernel<D, float><<<grid, PA_WAVES * 64, 0, ctx->stream>>>(a);
+  if (int s = check_launch(ctx, "paged_attention")) return s;
+  if (!cut) return MI_OK;
+  attend_join_kernel<D><<<static_cast<unsigned>(a.seqs * a.heads), 256, a.slots * sizeof(float), ctx->stream>>>(a);
+  return check_launch(ctx, "paged_attention join");
 }
 
 }  // namespace
@@ -338,13 +817,12 @@ extern "C" int mi_paged_attention(mi_ctx *ctx, mi_id q, mi_id k_pages, mi_id v_p
   if (heads > INT32_MAX / c.D || qb->rows != c.seqs || qb->cols != heads * c.D)
     return fail(ctx, MI_E_ARG, "paged_attention: q is [%lld, %lld], want [%lld, %lld * %lld]", (long long)qb->rows,
                 (long long)qb->cols, (long long)c.seqs, (long long)heads, (long long)c.D);
-  if (c.seqs * heads > INT32_MAX) return fail(ctx, MI_E_UNSUPPORTED, "paged_attention: grid too large");
   mi_id id;
   Buffer *ob;
   int s = new_buffer(ctx, c.seqs, heads * c.D, out_elem, &id, &ob);
   if (s) return s;
   if (c.seqs > 0) {
-    AttendArgs a;
+    AttendArgs a{};
     a.q = qb->ptr;
     a.k = c.k;
     a.v = c.v;
@@ -354,18 +832,24 @@ extern "C" int mi_paged_attention(mi_ctx *ctx, mi_id q, mi_id k_pages, mi_id v_p
     a.per = c.per;
     a.pages = c.pages;
     a.page = page;
+    a.div = page_div(static_cast<uint32_t>(page));
     a.heads = static_cast<int>(heads);
     a.kv_heads = static_cast<int>(kv_heads);
-    a.scale = scale;
+    a.group = a.heads / a.kv_heads;
+    a.tiles = (a.group + PA_HEADS - 1) / PA_HEADS;
+    a.live = a.group < PA_HEADS ? a.group : PA_HEADS;
+    a.q16 = qb->elem == MI_BF16;
+    a.out16 = out_elem == MI_BF16;
+    a.scale = scale * 1.4426950408889634f;
     a.out = ob->ptr;
     a.flags = flags(ctx);
+    const bool kv16 = c.elem == MI_BF16;
     switch (c.D) {
-      case 16: attend_types<16>(ctx, a, qb->elem, c.elem, out_elem); break;
-      case 32: attend_types<32>(ctx, a, qb->elem, c.elem, out_elem); break;
-      case 64: attend_types<64>(ctx, a, qb->elem, c.elem, out_elem); break;
-      default: attend_types<128>(ctx, a, qb->elem, c.elem, out_elem); break;
+      case 16: s = attend_launch<16>(ctx, a, kv16); break;
+      case 32: s = attend_launch<32>(ctx, a, kv16); break;
+      case 64: s = attend_launch<64>(ctx, a, kv16); break;
+      default: s = attend_launch<128>(ctx, a, kv16); break;
     }
-    s = check_launch(ctx, "paged_attention");
     if (s) { mi_free(ctx, id); return s; }
   }
   *out = id;

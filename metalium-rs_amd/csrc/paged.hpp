@@ -40,4 +40,42 @@ MI_HD int64_t paged_row(int64_t p, int64_t j, int64_t o, int64_t kv_heads, int64
 // A sequence's length as the attention reads it: one outside [0, cap] is 0.
 MI_HD int64_t paged_len(int64_t len, int64_t cap) { return len < 0 || len > cap ? 0 : len; }
 
+// n / d for 0 <= n < 2^31 without a division: q = (mulhi(n, m) + n) >> s with
+// 2^s the power of two at or above d and m = floor(2^32 (2^s - d) / d) + 1
+// (mulhi(n, m) < n < 2^31, so the sum holds in 32 bits).
+struct PageDiv {
+  uint32_t m, s;
+};
+inline PageDiv page_div(uint32_t d) {
+  uint32_t s = 0;
+  while ((uint64_t(1) << s) < d) ++s;
+  return PageDiv{static_cast<uint32_t>(((uint64_t(1) << 32) * ((uint64_t(1) << s) - d)) / d + 1), s};
+}
+MI_HD uint32_t page_of(uint32_t n, PageDiv d) {
+  return (static_cast<uint32_t>((static_cast<uint64_t>(n) * d.m) >> 32) + n) >> d.s;
+}
+
+// How the attention cuts the sequences: chunks of at most C positions, C the
+// least multiple of `unit` at which all sequences together make about
+// `target` chunks, so every chunk is nearly the same work whatever the
+// lengths; a sequence's chunks are of one length, an idle one has one (empty).
+// target >= 1; sum: the lengths' sum.  Each chunk but a sequence's last is
+// full: a sequence cut in n > 1 has more than (n - 1) C positions, so the
+// chunks of cut sequences are at most 2 sum / C <= 2 target + 2.
+MI_HD int64_t chunk_limit(int64_t sum, int64_t target, int64_t unit) {
+  return (static_cast<int64_t>(static_cast<double>(sum) / static_cast<double>(target)) / unit + 1) * unit;
+}
+MI_HD int32_t chunk_count(int32_t len, int64_t limit) {
+  if (len <= limit) return 1;
+  const uint32_t c = static_cast<uint32_t>(limit);
+  return static_cast<int32_t>((static_cast<uint32_t>(len) + c - 1) / c);
+}
+// The positions of each of a sequence's n chunks (the last may be shorter or
+// empty), a multiple of `unit`.
+MI_HD int32_t chunk_len(int32_t len, int32_t n, int32_t unit) {
+  if (n == 1) return len;
+  const uint32_t units = (static_cast<uint32_t>(len) + unit - 1) / unit;
+  return static_cast<int32_t>((units + n - 1) / n) * unit;
+}
+
 }  // namespace mi

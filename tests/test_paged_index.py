@@ -1,10 +1,12 @@
 """The index arithmetic of the paged KV cache, on the CPU: the header the
 kernels use, compiled for the host.  Whatever the lengths, bounds and rows say,
-a position that counts as good lies in what the table names, and rows of the
-pool are a bijection of (page, head, offset)."""
+a position that counts as good lies in what the table names, rows of the pool
+are a bijection of (page, head, offset), and the attention's chunks cover each
+sequence once, no more of them than the grid and the partials have room for."""
 import ctypes
 import itertools
 import os
+import random
 import subprocess
 
 import pytest
@@ -23,6 +25,11 @@ def lib(tmp_path_factory):
     I64 = ctypes.c_int64
     L.pos_of.argtypes = [I64] * 5 + [ctypes.POINTER(I64)]
     L.row_of.argtypes, L.row_of.restype = [I64] * 5, I64
+    U32, I32 = ctypes.c_uint32, ctypes.c_int32
+    L.quotient.argtypes, L.quotient.restype = [U32] * 2, U32
+    L.limit_of.argtypes, L.limit_of.restype = [I64] * 3, I64
+    L.count_of.argtypes = [I32, I64]
+    L.chunk_len_of.argtypes = [I32] * 3
     L.len_of.argtypes, L.len_of.restype = [I64] * 2, I64
     return L
 
@@ -72,3 +79,38 @@ def test_pool_rows_are_a_bijection(lib):
     assert rows == list(range(pages * kv * page))
     # Past 32 bits.
     assert lib.row_of(1 << 20, 7, 63, 8, 64) == ((1 << 20) * 8 + 7) * 64 + 63
+
+
+def test_quotients(lib):
+    rng = random.Random(1)
+    for d in [1, 2, 3, 5, 7, 15, 16, 17, 24, 48, 64, 640, 641, 65535, 65536, 2**30 - 1, 2**30, 2**30 + 1, I32_MAX] + \
+            [rng.randrange(1, I32_MAX) for _ in range(200)]:
+        ns = [0, 1, d - 1, d, 2 * d - 1, I32_MAX - 1, I32_MAX] + [rng.randrange(I32_MAX) for _ in range(20)]
+        ns += [k * d + e for k in (1, 2, I32_MAX // d) for e in (-1, 0, 1)]
+        for n in ns:
+            if 0 <= n <= I32_MAX:
+                assert lib.quotient(n, d) == n // d, (n, d)
+
+
+@pytest.mark.parametrize("unit", [64])
+def test_chunks_cover_each_sequence_within_bounds(lib, unit):
+    rng = random.Random(2)
+    cases = [[1], [0], [0] * 70, [64], [65], [I32_MAX], [I32_MAX] * 5, [100000] + [1] * 63, [1] * 3000]
+    for _ in range(300):
+        hi = 10 ** rng.randint(0, 9)
+        cases.append([rng.randint(0, hi) for _ in range(rng.randint(1, 80))])
+    for lens in cases:
+        for target in (1, 7, 128, 1024):
+            limit = lib.limit_of(sum(lens), target, unit)
+            assert limit % unit == 0 and limit >= unit
+            chunks = slots = 0
+            for n in lens:
+                c = lib.count_of(n, limit)
+                size = lib.chunk_len_of(n, c, unit)
+                assert c >= 1 and (c - 1) * limit <= n <= c * limit
+                assert c * size >= n and (c == 1 or (size % unit == 0 and size <= limit))
+                assert c <= max(1, -(-n // unit))
+                chunks += c
+                slots += c if c > 1 else 0
+            assert chunks <= target + 1 + len(lens)
+            assert slots <= 2 * target + 2
