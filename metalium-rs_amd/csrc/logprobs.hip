@@ -6,9 +6,12 @@
 // greedy pick of the generation loop (crates/tt-models/src/generate.rs:
 // 176-183), of which the alternatives are the ordered form.
 //
-// With z = scale x, m = max z, S = sum e^(z - m) and T = sum (z - m) e^(z - m):
-// lse = m + ln S, logp = z_target - lse, entropy = ln S - T / S (both terms
-// are at least 0, so nothing cancels).
+// With m = max x, c = scale log2(e), d = (x - m) c, S = sum 2^d and
+// T = sum d 2^d: lse = scale m + ln S, logp = ln 2 (d_target - log2 S),
+// entropy = ln 2 (log2 S - T / S), both terms at least 0.  The difference to
+// the maximum comes first, so a large common offset costs nothing and a row of
+// the type's lowest value does not overflow.
+#include <cfloat>
 #include <cmath>
 
 #include "common.hpp"
@@ -16,6 +19,35 @@
 
 namespace mi {
 namespace {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int LP_CAND = 1024;   // candidates for the alternatives a block holds
+constexpr int LP_TILES = 20;    // tiles a block takes of a row at most
+constexpr int LP_SLICES = 64;   // slices of a row at most: a wavefront's lanes rank them
+constexpr int64_t LP_BLOCKS = 512;  // rows below this are cut in slices
+
+// 16 bytes of a row: 4 F32 or 8 BF16 logits.
+template <typename T>
+struct Chunk16;
+template <>
+struct Chunk16<float> {
+  static constexpr int E = 4, MAX_NL = 8;
+  template <bool NT>
+  static __device__ __forceinline__ uint4 load(const float *p) { return ldu4<NT>(p); }
+  static __device__ __forceinline__ float get(const uint4 &v, int e) {
+    return __uint_as_float(e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w);
+  }
+};
+template <>
+struct Chunk16<uint16_t> {
+  static constexpr int E = 8, MAX_NL = 4;
+  template <bool NT>
+  static __device__ __forceinline__ uint4 load(const uint16_t *p) { return ldu4<NT>(p); }
+  static __device__ __forceinline__ float get(const uint4 &v, int e) {
+    const uint32_t w = e < 2 ? v.x : e < 4 ? v.y : e < 6 ? v.z : v.w;
+    return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+  }
+};
 
 __device__ __forceinline__ float logit(const float *p) { return *p; }
 __device__ __forceinline__ float logit(const uint16_t *p) { return bf16_bits_to_f32(*p); }
@@ -25,79 +57,401 @@ struct LogprobArgs {
   int64_t rows, cols;
   const int32_t *targets;
   float scale;
-  int top;
+  int top, slices;
+  int64_t slice;  // 16-byte chunks a slice
+  // Slices' statistics [rows][slices][4] and alternatives [rows][slices][top].
+  float *stats;
+  ArgBest *lists;
   float *logp, *lse, *entropy, *top_logp;
   int32_t *top_ids;
   uint32_t *flags;
 };
 
-// Whether (v, i) comes behind the pick `p` in the order of alternatives.
-__device__ __forceinline__ bool behind(float v, int32_t i, ArgBest p) {
-  const ArgBest b = better(ArgBest{v, i}, p);
-  return b.i == p.i && i != p.i;
+// The order of alternatives: the larger value first, a NaN above every
+// number, the lower column among equals (argmax's rule, as a comparison).
+__device__ __forceinline__ bool before(ArgBest a, ArgBest b) {
+  const bool an = isnan(a.v), bn = isnan(b.v);
+  if (an != bn) return an;
+  if (!an && a.v != b.v) return a.v > b.v;
+  return a.i < b.i;
+}
+
+// S and T of a maximum m moved to a maximum to >= m.
+__device__ __forceinline__ void rescale(float m, float to, float c, float &S, float &T) {
+  const float d = fmaxf((m - to) * c, -1e4f), r = __builtin_amdgcn_exp2f(d);
+  T = r * __builtin_fmaf(d, S, T);
+  S *= r;
+}
+// What distances are measured from: the largest logit, or a finite value where
+// all are -inf, so that those distances are -inf and not NaN.
+__device__ __forceinline__ float origin(float m) { return fmaxf(m, -FLT_MAX); }
+
+// The k-th largest of the lanes' values, equal ones counted as often as they
+// are there.
+__device__ __forceinline__ float kth_largest(float v, int k, int lane) {
+  int rank = 0;
+#pragma unroll 16
+  for (int o = 0; o < 64; ++o) {
+    const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), o));
+    rank += (w > v || (w == v && o < lane)) ? 1 : 0;
+  }
+  const uint64_t at = __ballot(rank == k - 1);
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), __ffsll(static_cast<unsigned long long>(at)) - 1));
+}
+
+// A row's results from its statistics over all columns.
+template <typename T>
+__device__ __forceinline__ void put_stats(const LogprobArgs &a, int64_t r, float m, float S, float Tm) {
+  const bool none = S == 0.0f;  // every logit is -inf
+  const float ls = __builtin_log2f(S);
+  if (a.lse) a.lse[r] = none ? -INFINITY : __builtin_fmaf(LN2, ls, m * a.scale);
+  if (a.entropy) a.entropy[r] = none ? 0.0f : LN2 * (ls - Tm / S);
+  if (a.logp) {
+    const int32_t g = a.targets[r];
+    const bool ok = g >= 0 && g < a.cols;
+    if (!ok) atomicOr(a.flags, FLAG_INDEX_RANGE);
+    const float x = logit(static_cast<const T *>(a.x) + r * a.cols + (ok ? g : 0));
+    a.logp[r] = !ok ? 0.0f : none ? -INFINITY : LN2 * ((x - m) * (a.scale * LOG2E) - ls);
+  }
+}
+__device__ __forceinline__ void put_top(const LogprobArgs &a, int64_t at, ArgBest b, float m, float S) {
+  a.top_logp[at] = S == 0.0f ? -INFINITY : LN2 * ((b.v - m) * (a.scale * LOG2E) - __builtin_log2f(S));
+  a.top_ids[at] = b.i;
+}
+
+// One slice of a row a block.  Its columns come in tiles of 256 threads x NL
+// chunks of 16 bytes, read once; a thread keeps the sums of its own columns
+// under its own running maximum and joins them with the others' at the end.
+//
+// Alternatives: the largest logit of each thread and tile stays in LDS.  The
+// k-th largest of 64 groups' maxima (four threads each) is a bound that at
+// least k columns reach, and only the few cells (thread, tile) that reach it
+// are looked at again -- from registers where the slice is one tile.  The
+// columns found, of the order of k, are ranked against each other.  More equal
+// columns than there is room for (a constant row) are taken in order from the
+// row's start; a row with a NaN or +inf, and one whose columns above the bound
+// are too many, is searched k times.
+template <typename T, int NL, bool TOP, bool NT>
+__global__ void __launch_bounds__(256) logprobs_kernel(LogprobArgs a) {
+  using C = Chunk16<T>;
+  constexpr int E = C::E;
+  __shared__ float red[4][3];
+  __shared__ float groups[64];
+  __shared__ ArgBest cand[TOP ? LP_CAND : 1];
+  __shared__ int count[2];  // candidates, and those above the bound
+  __shared__ ArgBest bests[4];
+  __shared__ float cells[TOP ? LP_TILES : 1][256];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t r = blockIdx.x / a.slices;
+  const int sl = static_cast<int>(blockIdx.x % a.slices);
+  // The row from the 16-byte boundary at or before it: column c is element
+  // c + skip.
+  const int64_t flat = r * a.cols;
+  const int skip = static_cast<int>(flat & (E - 1));
+  const T *x = static_cast<const T *>(a.x) + (flat - skip);
+  const int64_t end = a.cols + skip, chunks = (end + E - 1) / E;
+  const int64_t c0 = sl * a.slice, c1 = c0 + a.slice < chunks ? c0 + a.slice : chunks;
+  const float c = a.scale * LOG2E;
+  if (TOP && tid < 2) count[tid] = 0;
+
+  uint4 v[NL], nx[NL];
+  auto load = [&](int64_t t0, uint4 (&w)[NL]) {
+#pragma unroll
+    for (int u = 0; u < NL; ++u) {
+      const int64_t q = t0 + u * 256 + tid;
+      w[u] = C::template load<NT>(x + (q < c1 ? q : c1 - 1) * E);
+    }
+  };
+  // Whether element e of the chunk at q is a column of this slice.
+  auto mine = [&](int64_t q, int e) { return q < c1 && q * E + e >= skip && q * E + e < end; };
+
+  float mx = -INFINITY, m = -FLT_MAX, S = 0.0f, Tm = 0.0f;
+  int tiles = 0;
+  load(c0, v);
+  for (int64_t t0 = c0; t0 < c1; t0 += 256 * NL, ++tiles) {
+    const bool more = t0 + 256 * NL < c1;
+    if (more) load(t0 + 256 * NL, nx);
+    float xs[NL][E];
+    float tm = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < NL; ++u)
+#pragma unroll
+      for (int e = 0; e < E; ++e) xs[u][e] = C::get(v[u], e);
+    if (t0 == 0 || !more) {  // elements outside the slice lie in its ends' tiles
+#pragma unroll
+      for (int u = 0; u < NL; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e) xs[u][e] = mine(t0 + u * 256 + tid, e) ? xs[u][e] : -INFINITY;
+    }
+#pragma unroll
+    for (int u = 0; u < NL; ++u)
+#pragma unroll
+      for (int e = 0; e < E; ++e) tm = fmaxf(tm, xs[u][e]);
+    if (TOP) cells[tiles][tid] = tm;
+    if (tm > mx) {
+      mx = tm;
+      rescale(m, origin(mx), c, S, Tm);
+      m = origin(mx);
+    }
+#pragma unroll
+    for (int u = 0; u < NL; ++u)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float d = (xs[u][e] - m) * c, w = __builtin_amdgcn_exp2f(d);
+        S += w;
+        Tm = __builtin_fmaf(fmaxf(d, -1e4f), w, Tm);  // 2^-inf = 0 adds nothing
+      }
+    if (more) {
+#pragma unroll
+      for (int u = 0; u < NL; ++u) v[u] = nx[u];
+    }
+  }
+
+  // The block's maximum, then its sums.
+  float M = fold_max<64>(mx);
+  if (lane == 0) red[wave][0] = M;
+  if (TOP) {
+    const float gm = fold_max<4>(mx);
+    if ((lane & 3) == 0) groups[tid >> 2] = gm;
+  }
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
+  M = origin(M);
+  rescale(m, M, c, S, Tm);
+  S = fold_sum<64>(S);
+  Tm = fold_sum<64>(Tm);
+  if (lane == 0) {
+    red[wave][1] = S;
+    red[wave][2] = Tm;
+  }
+  __syncthreads();
+  S = (red[0][1] + red[1][1]) + (red[2][1] + red[3][1]);
+  Tm = (red[0][2] + red[1][2]) + (red[2][2] + red[3][2]);
+  if (tid == 0) {
+    if (a.slices == 1) {
+      put_stats<T>(a, r, M, S, Tm);
+    } else {
+      float *st = a.stats + (r * a.slices + sl) * 4;
+      st[0] = M;
+      st[1] = S;
+      st[2] = Tm;
+    }
+  }
+  if constexpr (!TOP) return;
+
+  const int k = a.top;
+  ArgBest *list = a.slices > 1 ? a.lists + (r * a.slices + sl) * k : nullptr;
+  auto put = [&](int at, ArgBest b) {
+    if (list) list[at] = b;
+    else put_top(a, r * k + at, b, M, S);
+  };
+  const int64_t e0 = c0 * E > skip ? c0 * E - skip : 0;  // the slice's columns [e0, e1)
+  const int64_t e1 = c1 * E - skip < a.cols ? c1 * E - skip : a.cols;
+  bool search = isnan(S);
+  int n = 0, above = 0;
+  float bound = -INFINITY;
+  if (!search) {
+    bound = kth_largest(groups[lane], k, lane);
+    auto offer = [&](int64_t q, int e, float w) {
+      if (w >= bound && mine(q, e)) {
+        if (w > bound) atomicAdd(&count[1], 1);
+        const int at = atomicAdd(&count[0], 1);
+        if (at < LP_CAND) cand[at] = ArgBest{w, static_cast<int32_t>(q * E + e - skip)};
+      }
+    };
+    if (mx >= bound) {
+      for (int t = 0; t < tiles; ++t) {
+        if (!(cells[t][tid] >= bound)) continue;
+        const int64_t t0 = c0 + static_cast<int64_t>(t) * 256 * NL;
+        if (tiles > 1) load(t0, v);
+#pragma unroll
+        for (int u = 0; u < NL; ++u)
+#pragma unroll
+          for (int e = 0; e < E; ++e) offer(t0 + u * 256 + tid, e, C::get(v[u], e));
+      }
+    }
+    __syncthreads();
+    n = count[0];
+    above = count[1];
+    __syncthreads();
+  }
+  if (!search && n > LP_CAND) {
+    if (above > LP_CAND - k) {
+      search = true;
+    } else {
+      // The columns above the bound (fewer than k), then the first ones equal
+      // to it.
+      if (tid < 2) count[tid] = 0;
+      __syncthreads();
+      const T *row = x + skip;
+      for (int64_t b = e0; b < e1; b += 256) {
+        const float w = b + tid < e1 ? logit(row + b + tid) : -INFINITY;
+        if (b + tid < e1 && w > bound) {
+          const int at = atomicAdd(&count[0], 1);
+          cand[at] = ArgBest{w, static_cast<int32_t>(b + tid)};
+        }
+      }
+      __syncthreads();
+      n = count[0];
+      for (int64_t b = e0; b < e1 && n < above + k; b += 256) {
+        const bool eq = b + tid < e1 && logit(row + b + tid) == bound;
+        const uint64_t bal = __ballot(eq);
+        if (lane == 0) red[wave][0] = static_cast<float>(__popcll(bal));
+        __syncthreads();
+        int at = n + __popcll(bal & ((uint64_t(1) << lane) - 1)), all = 0;
+        for (int w = 0; w < 4; ++w) {
+          const int cw = static_cast<int>(red[w][0]);
+          if (w < wave) at += cw;
+          all += cw;
+        }
+        if (eq && at < LP_CAND) cand[at] = ArgBest{bound, static_cast<int32_t>(b + tid)};
+        n += all;
+        __syncthreads();
+      }
+      if (n > LP_CAND) n = LP_CAND;
+    }
+  }
+  if (search) {
+    const T *row = x + skip;
+    ArgBest last{0.0f, -1};
+    for (int t = 0; t < k; ++t) {
+      ArgBest b{0.0f, -1};
+      for (int64_t q = e0 + tid; q < e1; q += 256) {
+        const ArgBest w{logit(row + q), static_cast<int32_t>(q)};
+        if (t > 0 && !before(last, w)) continue;
+        if (b.i < 0 || before(w, b)) b = w;
+      }
+      for (int o = 32; o >= 1; o >>= 1) {
+        const ArgBest w{__shfl_xor(b.v, o, 64), __shfl_xor(b.i, o, 64)};
+        if (b.i < 0 || (w.i >= 0 && before(w, b))) b = w;
+      }
+      if (lane == 0) bests[wave] = b;
+      __syncthreads();
+      last = bests[0];
+      for (int w = 1; w < 4; ++w)
+        if (last.i < 0 || (bests[w].i >= 0 && before(bests[w], last))) last = bests[w];
+      __syncthreads();
+      // A slice of fewer columns: entries behind every column.
+      if (last.i < 0) last = ArgBest{-INFINITY, INT32_MAX};
+      if (tid == 0) put(t, last);
+    }
+    return;
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += 256) {
+    const ArgBest b = cand[i];
+    int rank = 0;
+    for (int o = 0; o < n; ++o) rank += cand[o].v > b.v || (cand[o].v == b.v && cand[o].i < b.i) ? 1 : 0;
+    if (rank < k) put(rank, b);
+  }
+  for (int i = n + tid; i < k; i += 256) put(i, ArgBest{-INFINITY, INT32_MAX});
+}
+
+// Joins the slices of a row.
+template <typename T>
+__global__ void __launch_bounds__(256) logprobs_join_kernel(LogprobArgs a) {
+  __shared__ ArgBest cand[LP_SLICES * MI_TOP_MAX];
+  __shared__ int count;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int64_t r = blockIdx.x;
+  const int ns = a.slices, k = a.top;
+  const float *st = a.stats + r * ns * 4;
+  const float m = lane < ns ? st[lane * 4] : -FLT_MAX;
+  float S = lane < ns ? st[lane * 4 + 1] : 0.0f, Tm = lane < ns ? st[lane * 4 + 2] : 0.0f;
+  const float M = fold_max<64>(m);
+  rescale(m, M, a.scale * LOG2E, S, Tm);
+  S = fold_sum<64>(S);
+  Tm = fold_sum<64>(Tm);
+  if (tid == 0) put_stats<T>(a, r, M, S, Tm);
+  if (k == 0) return;
+  const ArgBest *lists = a.lists + r * ns * k;
+  const int all = ns * k;
+  // A column before the k-th best of the slices' first ones is among the
+  // first k; the others need not be ranked.
+  ArgBest bound{-INFINITY, INT32_MAX};
+  if (ns >= k) {
+    const ArgBest f = lane < ns ? lists[lane * k] : bound;
+    int rank = 0;
+    for (int o = 0; o < ns; ++o) {
+      const ArgBest w{__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f.v), o)),
+                      __builtin_amdgcn_readlane(f.i, o)};
+      rank += before(w, f) ? 1 : 0;
+    }
+    const uint64_t at = __ballot(lane < ns && rank == k - 1);
+    if (at) {
+      const int l = __ffsll(static_cast<unsigned long long>(at)) - 1;
+      bound = ArgBest{__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f.v), l)),
+                      __builtin_amdgcn_readlane(f.i, l)};
+    }
+  }
+  if (tid == 0) count = 0;
+  __syncthreads();
+  for (int i = tid; i < all; i += 256) {
+    const ArgBest b = lists[i];
+    if (b.i != INT32_MAX && !before(bound, b)) cand[atomicAdd(&count, 1)] = b;
+  }
+  __syncthreads();
+  const int n = count;
+  for (int i = tid; i < n; i += 256) {
+    const ArgBest b = cand[i];
+    int rank = 0;
+    for (int o = 0; o < n; ++o) rank += before(cand[o], b) ? 1 : 0;
+    if (rank < k) put_top(a, r * k + rank, b, M, S);
+  }
+}
+
+template <typename T, int NL, bool TOP>
+void logprobs_launch(Ctx *ctx, const LogprobArgs &a, bool nt) {
+  const unsigned grid = static_cast<unsigned>(a.rows * a.slices);
+  if (nt) logprobs_kernel<T, NL, TOP, true><<<grid, 256, 0, ctx->stream>>>(a);
+  else logprobs_kernel<T, NL, TOP, false><<<grid, 256, 0, ctx->stream>>>(a);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) logprobs_kernel(LogprobArgs a) {
-  __shared__ float red[4][2];
-  __shared__ ArgBest bests[4];
-  const int64_t r = blockIdx.x;
-  const T *x = static_cast<const T *>(a.x) + r * a.cols;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  float m = -INFINITY;
-  for (int64_t c = tid; c < a.cols; c += 256) m = max_nan(m, logit(x + c) * a.scale);
-  m = fold_max<64>(m);
-  if (lane == 0) red[wave][0] = m;
-  __syncthreads();
-  m = max_nan(max_nan(red[0][0], red[1][0]), max_nan(red[2][0], red[3][0]));
-  __syncthreads();
-  float s = 0.0f, t = 0.0f;
-  for (int64_t c = tid; c < a.cols; c += 256) {
-    const float d = logit(x + c) * a.scale - m, e = expf(d);
-    s += e;
-    t += e == 0.0f ? 0.0f : d * e;
+int logprobs_run(Ctx *ctx, LogprobArgs a) {
+  using C = Chunk16<T>;
+  constexpr int64_t TILE = 256 * C::MAX_NL;
+  const int64_t chunks = (a.cols + 2 * (C::E - 1)) / C::E;  // of a row that starts anywhere
+  int64_t ns = 1;
+  if (a.rows < LP_BLOCKS && chunks > TILE) {
+    const int64_t want = (LP_BLOCKS + a.rows - 1) / a.rows, most = (chunks + 255) / 256;
+    ns = want < most ? want : most;
+    if (ns > LP_SLICES) ns = LP_SLICES;
   }
-  s = fold_sum<64>(s);
-  t = fold_sum<64>(t);
-  if (lane == 0) { red[wave][0] = s; red[wave][1] = t; }
-  __syncthreads();
-  s = (red[0][0] + red[1][0]) + (red[2][0] + red[3][0]);
-  t = (red[0][1] + red[1][1]) + (red[2][1] + red[3][1]);
-  const bool none = m == -INFINITY;  // every logit is -inf
-  const float lse = none ? -INFINITY : m + logf(s);
-  if (tid == 0) {
-    if (a.lse) a.lse[r] = lse;
-    if (a.entropy) a.entropy[r] = none ? 0.0f : logf(s) - t / s;
-    if (a.logp) {
-      const int32_t g = a.targets[r];
-      const bool ok = g >= 0 && g < a.cols;
-      if (!ok) atomicOr(a.flags, FLAG_INDEX_RANGE);
-      a.logp[r] = !ok ? 0.0f : none ? -INFINITY : logit(x + g) * a.scale - lse;
-    }
+  const int64_t least = (chunks + LP_TILES * TILE - 1) / (LP_TILES * TILE);
+  if (ns < least) ns = least;
+  a.slice = (chunks + ns - 1) / ns;
+  // Every slice holds a column of every row: the shortest row's chunks.
+  const int64_t shortest = (a.cols + C::E - 1) / C::E;
+  ns = (shortest + a.slice - 1) / a.slice;
+  if (ns * a.slice < chunks) a.slice = (chunks + ns - 1) / ns;
+  if (ns > LP_SLICES || a.slice > LP_TILES * TILE || a.rows * ns > INT32_MAX)
+    return fail(ctx, MI_E_UNSUPPORTED, "token_logprobs of [%lld, %lld]", (long long)a.rows, (long long)a.cols);
+  a.slices = static_cast<int>(ns);
+  if (ns > 1) {
+    const size_t cells = static_cast<size_t>(a.rows * ns);
+    char *p = static_cast<char *>(scratch(ctx, cells * (16 + sizeof(ArgBest) * a.top)));
+    if (!p) return fail(ctx, MI_E_OOM, "token_logprobs scratch");
+    a.stats = reinterpret_cast<float *>(p);
+    a.lists = reinterpret_cast<ArgBest *>(p + cells * 16);
   }
-  ArgBest last{0.0f, -1};
-  for (int k = 0; k < a.top; ++k) {
-    ArgBest b{0.0f, -1};
-    for (int64_t c = tid; c < a.cols; c += 256) {
-      const float v = logit(x + c);
-      const int32_t i = static_cast<int32_t>(c);
-      if (k > 0 && !behind(v, i, last)) continue;
-      b = b.i < 0 ? ArgBest{v, i} : better(b, ArgBest{v, i});
-    }
-    for (int o = 32; o >= 1; o >>= 1) {
-      const ArgBest n{__shfl_xor(b.v, o, 64), __shfl_xor(b.i, o, 64)};
-      b = n.i < 0 ? b : b.i < 0 ? n : better(b, n);
-    }
-    __syncthreads();
-    if (lane == 0) bests[wave] = b;
-    __syncthreads();
-    last = bests[0];
-    for (int w = 1; w < 4; ++w) last = bests[w].i < 0 ? last : last.i < 0 ? bests[w] : better(last, bests[w]);
-    if (tid == 0) {
-      a.top_logp[r * a.top + k] = none ? -INFINITY : last.v * a.scale - lse;
-      a.top_ids[r * a.top + k] = last.i;
-    }
+  const bool nt = a.rows * a.cols * static_cast<int64_t>(sizeof(T)) >= kStreamBytes;
+  const int nl = a.slice <= 256 ? 1 : a.slice <= 512 ? 2 : a.slice <= 1024 ? 4 : C::MAX_NL;
+  if (a.top > 0) {
+    if (nl == 1) logprobs_launch<T, 1, true>(ctx, a, nt);
+    else if (nl == 2) logprobs_launch<T, 2, true>(ctx, a, nt);
+    else if (nl == 4) logprobs_launch<T, 4, true>(ctx, a, nt);
+    else logprobs_launch<T, C::MAX_NL, true>(ctx, a, nt);
+  } else {
+    if (nl == 1) logprobs_launch<T, 1, false>(ctx, a, nt);
+    else if (nl == 2) logprobs_launch<T, 2, false>(ctx, a, nt);
+    else if (nl == 4) logprobs_launch<T, 4, false>(ctx, a, nt);
+    else logprobs_launch<T, C::MAX_NL, false>(ctx, a, nt);
   }
+  if (int s = check_launch(ctx, "token_logprobs")) return s;
+  if (ns == 1) return MI_OK;
+  logprobs_join_kernel<T><<<static_cast<unsigned>(a.rows), 256, 0, ctx->stream>>>(a);
+  return check_launch(ctx, "token_logprobs join");
 }
 
 struct LogprobGradArgs {
@@ -107,37 +461,104 @@ struct LogprobGradArgs {
   const float *lse, *entropy, *d_logp, *d_entropy;
   float scale;
   void *out;
+  int blocks;  // a row
   uint32_t *flags;
 };
 
-// dx_j = scale (g ([j = target] - p_j) - h p_j (z_j - lse + H)).
-template <typename T, typename TO>
+// e^l for l <= 0 or so from the hardware's 2^y, y = l log2(e) rounded: what
+// the rounding and the constant's own leave out (log2(e) = LOG2E + LOG2E_LO)
+// goes into a factor 1 + r, so the error does not grow with |l| (without it
+// 2.2 |l| 2^-24 of the value).
+__device__ __forceinline__ float exp_neg(float l) {
+  constexpr float LOG2E_LO = 1.925963033500e-8f;
+  const float y = l * LOG2E, p = __builtin_amdgcn_exp2f(y);
+  const float r = LN2 * __builtin_fmaf(l, LOG2E_LO, __builtin_fmaf(l, LOG2E, -y));
+  return p == 0.0f ? 0.0f : __builtin_fmaf(p, r, p);
+}
+
+// dx_j = scale (g ([j = target] - p_j) - h p_j (z_j - lse + H)), eight
+// elements a thread and turn, from a 16-byte boundary of both sides at or
+// before the row: one read and one write of each byte, bound by HBM.
+template <typename T, typename TO, bool NT>
 __global__ void __launch_bounds__(256) logprobs_backward_kernel(LogprobGradArgs a) {
-  const int64_t r = blockIdx.x;
-  const T *x = static_cast<const T *>(a.x) + r * a.cols;
-  TO *o = static_cast<TO *>(a.out) + r * a.cols;
+  const int64_t r = blockIdx.x / a.blocks;
+  const int blk = static_cast<int>(blockIdx.x % a.blocks);
+  const int64_t flat = r * a.cols;
+  const int skip = static_cast<int>(flat & 7);
+  const T *x = static_cast<const T *>(a.x) + (flat - skip);
+  TO *o = static_cast<TO *>(a.out) + (flat - skip);
+  const int64_t end = a.cols + skip, chunks = (end + 7) / 8;
   const float lse = a.lse[r], h = a.d_entropy ? a.d_entropy[r] : 0.0f, H = a.d_entropy ? a.entropy[r] : 0.0f;
   float g = a.d_logp ? a.d_logp[r] : 0.0f;
-  int32_t target = -1;
+  int64_t target = -1;
   if (a.d_logp) {
     target = a.targets[r];
     if (target < 0 || target >= a.cols) {
-      if (threadIdx.x == 0) atomicOr(a.flags, FLAG_INDEX_RANGE);
+      if (threadIdx.x == 0 && blk == 0) atomicOr(a.flags, FLAG_INDEX_RANGE);
       target = -1;
       g = 0.0f;
     }
   }
-  for (int64_t c = threadIdx.x; c < a.cols; c += 256) {
-    const float l = lse == -INFINITY ? -INFINITY : logit(x + c) * a.scale - lse, p = expf(l);
-    const float w = p == 0.0f ? 0.0f : p * (g + h * (l + H));
-    f32_put(o + c, ((c == target ? g : 0.0f) - w) * a.scale);
+  const bool none = lse == -INFINITY;
+  if (target >= 0) target += skip;
+  for (int64_t q = static_cast<int64_t>(blk) * 256 + threadIdx.x; q < chunks; q += static_cast<int64_t>(a.blocks) * 256) {
+    float v[8];
+    if constexpr (sizeof(T) == 2) {
+      const uint4 w = ldu4<NT>(x + 8 * q);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = Chunk16<uint16_t>::get(w, e);
+    } else {
+      // The second half of a row's last chunk may lie past the buffer.
+      const bool two = 8 * q + 4 < end;
+      const uint4 w = ldu4<NT>(x + 8 * q), y = ldu4<NT>(x + 8 * q + (two ? 4 : 0));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = Chunk16<float>::get(w, e);
+        v[4 + e] = Chunk16<float>::get(y, e);
+      }
+    }
+    float out[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float l = __builtin_fmaf(v[e], a.scale, -lse), p = none ? 0.0f : exp_neg(l);
+      // 0 times a finite bracket where the probability is 0.
+      const float w = p * __builtin_fmaf(h, fmaxf(l, -1e4f) + H, g);
+      out[e] = ((8 * q + e == target ? g : 0.0f) - w) * a.scale;
+    }
+    if (8 * q >= skip && 8 * q + 8 <= end) {
+      if constexpr (sizeof(TO) == 2) {
+        stu4<NT>(o + 8 * q, make_uint4(bf16x2_bits(out[0], out[1]), bf16x2_bits(out[2], out[3]),
+                                       bf16x2_bits(out[4], out[5]), bf16x2_bits(out[6], out[7])));
+      } else {
+        st4<NT>(o + 8 * q, make_float4(out[0], out[1], out[2], out[3]));
+        st4<NT>(o + 8 * q + 4, make_float4(out[4], out[5], out[6], out[7]));
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (8 * q + e >= skip && 8 * q + e < end) f32_put(o + 8 * q + e, out[e]);
+    }
   }
+}
+
+template <typename T, typename TO>
+void logprobs_backward_launch(Ctx *ctx, LogprobGradArgs a) {
+  const bool nt = a.rows * a.cols * static_cast<int64_t>(sizeof(T) + sizeof(TO)) >= kStreamBytes;
+  // Four turns a thread, fewer where the rows are few.
+  const int64_t chunks = (a.cols + 14) / 8;
+  int64_t per = (chunks + 1023) / 1024;
+  if (a.rows * per < 1024) per = (1024 + a.rows - 1) / a.rows;
+  const int64_t most = (chunks + 255) / 256;
+  a.blocks = static_cast<int>(per < most ? per : most);
+  const unsigned grid = static_cast<unsigned>(a.rows * a.blocks);
+  if (nt) logprobs_backward_kernel<T, TO, true><<<grid, 256, 0, ctx->stream>>>(a);
+  else logprobs_backward_kernel<T, TO, false><<<grid, 256, 0, ctx->stream>>>(a);
 }
 
 int logits_check(Ctx *ctx, const char *what, const Buffer *xb, float scale) {
   if (!elem_float(xb->elem) || xb->tiles)
     return fail(ctx, MI_E_ARG, "%s takes F32 or BF16 logits in rows (%s)", what, elem_name(xb->elem));
-  if (xb->cols < 1 || xb->cols > INT32_MAX || xb->rows > INT32_MAX)
+  if (xb->cols < 1 || xb->cols >= INT32_MAX || xb->rows > INT32_MAX)
     return fail(ctx, MI_E_ARG, "%s of [%lld, %lld]", what, (long long)xb->rows, (long long)xb->cols);
   if (!(scale > 0.0f) || std::isinf(scale))
     return fail(ctx, MI_E_ARG, "%s: scale %g (positive and finite)", what, static_cast<double>(scale));
@@ -201,10 +622,7 @@ extern "C" int mi_token_logprobs(mi_ctx *ctx, mi_id logits, mi_id targets, float
     a.entropy = static_cast<float *>(ptrs[2]);
     a.top_logp = static_cast<float *>(ptrs[3]);
     a.top_ids = static_cast<int32_t *>(ptrs[4]);
-    const unsigned grid = static_cast<unsigned>(R);
-    if (xb->elem == MI_BF16) logprobs_kernel<uint16_t><<<grid, 256, 0, ctx->stream>>>(a);
-    else logprobs_kernel<float><<<grid, 256, 0, ctx->stream>>>(a);
-    s = check_launch(ctx, "token_logprobs");
+    s = xb->elem == MI_BF16 ? logprobs_run<uint16_t>(ctx, a) : logprobs_run<float>(ctx, a);
   }
   if (s) {
     for (mi_id id : ids)
@@ -259,12 +677,11 @@ extern "C" int mi_token_logprobs_backward(mi_ctx *ctx, mi_id logits, mi_id targe
   if (s) return s;
   a.out = ob->ptr;
   if (R > 0) {
-    const unsigned grid = static_cast<unsigned>(R);
     const bool x16 = xb->elem == MI_BF16, o16 = out_elem == MI_BF16;
-    if (x16 && o16) logprobs_backward_kernel<uint16_t, uint16_t><<<grid, 256, 0, ctx->stream>>>(a);
-    else if (x16) logprobs_backward_kernel<uint16_t, float><<<grid, 256, 0, ctx->stream>>>(a);
-    else if (o16) logprobs_backward_kernel<float, uint16_t><<<grid, 256, 0, ctx->stream>>>(a);
-    else logprobs_backward_kernel<float, float><<<grid, 256, 0, ctx->stream>>>(a);
+    if (x16 && o16) logprobs_backward_launch<uint16_t, uint16_t>(ctx, a);
+    else if (x16) logprobs_backward_launch<uint16_t, float>(ctx, a);
+    else if (o16) logprobs_backward_launch<float, uint16_t>(ctx, a);
+    else logprobs_backward_launch<float, float>(ctx, a);
     s = check_launch(ctx, "token_logprobs_backward");
     if (s) { mi_free(ctx, id); return s; }
   }

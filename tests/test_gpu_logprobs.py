@@ -150,6 +150,7 @@ def test_masked_logits(eng, cols, elem):
     x[2, rng.random(cols) < 0.95] = -np.inf
     x[3, rng.random(cols) < 0.5] = -3.3e38
     x[3, 17] = 1.0
+    x[4] = -3.3e38                      # all at the lowest values: uniform
     check(eng, x, elem, 1.0, 32, targets=[0, 0, 17, 17, 3])
 
 
