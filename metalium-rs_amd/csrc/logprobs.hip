@@ -61,19 +61,42 @@ struct LogprobArgs {
   int64_t slice;  // 16-byte chunks a slice
   // Slices' statistics [rows][slices][4] and alternatives [rows][slices][top].
   float *stats;
-  ArgBest *lists;
+  uint64_t *lists;
   float *logp, *lse, *entropy, *top_logp;
   int32_t *top_ids;
   uint32_t *flags;
 };
 
-// The order of alternatives: the larger value first, a NaN above every
-// number, the lower column among equals (argmax's rule, as a comparison).
-__device__ __forceinline__ bool before(ArgBest a, ArgBest b) {
-  const bool an = isnan(a.v), bn = isnan(b.v);
-  if (an != bn) return an;
-  if (!an && a.v != b.v) return a.v > b.v;
-  return a.i < b.i;
+// A logit and its column as one whole number that grows in the order of
+// alternatives (argmax's rule): the larger value first, 0 and -0 alike, a NaN
+// above every number, the lower column among equals.  0 stands for none.
+__device__ __forceinline__ uint64_t key_of(float v, int64_t col) {
+  const uint32_t b = __float_as_uint(v + 0.0f);
+  const uint32_t o = isnan(v) ? 0xffffffffu : b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+  return static_cast<uint64_t>(o) << 32 | (0xffffffffu - static_cast<uint32_t>(col));
+}
+__device__ __forceinline__ float key_value(uint64_t k) {
+  const uint32_t o = static_cast<uint32_t>(k >> 32);
+  return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);  // 0xffffffff: a NaN
+}
+__device__ __forceinline__ int32_t key_column(uint64_t k) {
+  return static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(k));
+}
+__device__ __forceinline__ uint64_t lane_key(uint64_t k, int lane) {
+  return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(k >> 32), lane))) << 32 |
+         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(k), lane));
+}
+// How many of the n keys are above k (keys padded with a 0 to an even number,
+// two a 16-byte read).
+__device__ __forceinline__ int rank_of(const uint64_t *keys, int n, uint64_t k) {
+  const ulonglong2 *p = reinterpret_cast<const ulonglong2 *>(keys);
+  int rank = 0;
+#pragma unroll 8
+  for (int o = 0; o < (n + 1) / 2; ++o) {
+    const ulonglong2 w = p[o];
+    rank += (w.x > k ? 1 : 0) + (w.y > k ? 1 : 0);
+  }
+  return rank;
 }
 
 // S and T of a maximum m moved to a maximum to >= m.
@@ -114,9 +137,9 @@ __device__ __forceinline__ void put_stats(const LogprobArgs &a, int64_t r, float
     a.logp[r] = !ok ? 0.0f : none ? -INFINITY : LN2 * ((x - m) * (a.scale * LOG2E) - ls);
   }
 }
-__device__ __forceinline__ void put_top(const LogprobArgs &a, int64_t at, ArgBest b, float m, float S) {
-  a.top_logp[at] = S == 0.0f ? -INFINITY : LN2 * ((b.v - m) * (a.scale * LOG2E) - __builtin_log2f(S));
-  a.top_ids[at] = b.i;
+__device__ __forceinline__ void put_top(const LogprobArgs &a, int64_t at, uint64_t key, float m, float S) {
+  a.top_logp[at] = S == 0.0f ? -INFINITY : LN2 * ((key_value(key) - m) * (a.scale * LOG2E) - __builtin_log2f(S));
+  a.top_ids[at] = key_column(key);
 }
 
 // One slice of a row a block.  Its columns come in tiles of 256 threads x NL
@@ -137,9 +160,9 @@ __global__ void __launch_bounds__(256) logprobs_kernel(LogprobArgs a) {
   constexpr int E = C::E;
   __shared__ float red[4][3];
   __shared__ float groups[64];
-  __shared__ ArgBest cand[TOP ? LP_CAND : 1];
-  __shared__ int count[2];  // candidates, and those above the bound
-  __shared__ ArgBest bests[4];
+  __shared__ __align__(16) uint64_t cand[TOP ? LP_CAND : 2];
+  __shared__ int count;
+  __shared__ uint64_t bests[4];
   __shared__ float cells[TOP ? LP_TILES : 1][256];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t r = blockIdx.x / a.slices;
@@ -152,7 +175,7 @@ __global__ void __launch_bounds__(256) logprobs_kernel(LogprobArgs a) {
   const int64_t end = a.cols + skip, chunks = (end + E - 1) / E;
   const int64_t c0 = sl * a.slice, c1 = c0 + a.slice < chunks ? c0 + a.slice : chunks;
   const float c = a.scale * LOG2E;
-  if (TOP && tid < 2) count[tid] = 0;
+  if (TOP && tid == 0) count = 0;
 
   uint4 v[NL], nx[NL];
   auto load = [&](int64_t t0, uint4 (&w)[NL]) {
@@ -240,60 +263,61 @@ __global__ void __launch_bounds__(256) logprobs_kernel(LogprobArgs a) {
   if constexpr (!TOP) return;
 
   const int k = a.top;
-  ArgBest *list = a.slices > 1 ? a.lists + (r * a.slices + sl) * k : nullptr;
-  auto put = [&](int at, ArgBest b) {
-    if (list) list[at] = b;
-    else put_top(a, r * k + at, b, M, S);
+  uint64_t *list = a.slices > 1 ? a.lists + (r * a.slices + sl) * k : nullptr;
+  auto put = [&](int at, uint64_t key) {
+    if (list) list[at] = key;
+    else put_top(a, r * k + at, key, M, S);
   };
   const int64_t e0 = c0 * E > skip ? c0 * E - skip : 0;  // the slice's columns [e0, e1)
   const int64_t e1 = c1 * E - skip < a.cols ? c1 * E - skip : a.cols;
+  const T *row = x + skip;
   bool search = isnan(S);
-  int n = 0, above = 0;
+  int n = 0;
   float bound = -INFINITY;
   if (!search) {
     bound = kth_largest(groups[lane], k, lane);
-    auto offer = [&](int64_t q, int e, float w) {
-      if (w >= bound && mine(q, e)) {
-        if (w > bound) atomicAdd(&count[1], 1);
-        const int at = atomicAdd(&count[0], 1);
-        if (at < LP_CAND) cand[at] = ArgBest{w, static_cast<int32_t>(q * E + e - skip)};
-      }
-    };
     if (mx >= bound) {
       for (int t = 0; t < tiles; ++t) {
         if (!(cells[t][tid] >= bound)) continue;
         const int64_t t0 = c0 + static_cast<int64_t>(t) * 256 * NL;
         if (tiles > 1) load(t0, v);
+        uint32_t hits = 0;
 #pragma unroll
         for (int u = 0; u < NL; ++u)
 #pragma unroll
-          for (int e = 0; e < E; ++e) offer(t0 + u * 256 + tid, e, C::get(v[u], e));
+          for (int e = 0; e < E; ++e)
+            hits |= (C::get(v[u], e) >= bound && mine(t0 + u * 256 + tid, e) ? 1u : 0u) << (u * E + e);
+        int at = atomicAdd(&count, __popc(hits));
+#pragma unroll
+        for (int u = 0; u < NL; ++u)
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (hits >> (u * E + e) & 1u) {
+              if (at < LP_CAND) cand[at] = key_of(C::get(v[u], e), (t0 + u * 256 + tid) * E + e - skip);
+              ++at;
+            }
       }
     }
     __syncthreads();
-    n = count[0];
-    above = count[1];
-    __syncthreads();
-  }
-  if (!search && n > LP_CAND) {
-    if (above > LP_CAND - k) {
-      search = true;
-    } else {
-      // The columns above the bound (fewer than k), then the first ones equal
-      // to it.
-      if (tid < 2) count[tid] = 0;
+    n = count;
+    if (n > LP_CAND) {
+      // More than there is room for.  The columns above the bound alone (where
+      // all are equal there is none), then the first ones equal to it.
       __syncthreads();
-      const T *row = x + skip;
-      for (int64_t b = e0; b < e1; b += 256) {
-        const float w = b + tid < e1 ? logit(row + b + tid) : -INFINITY;
-        if (b + tid < e1 && w > bound) {
-          const int at = atomicAdd(&count[0], 1);
-          cand[at] = ArgBest{w, static_cast<int32_t>(b + tid)};
+      if (tid == 0) count = 0;
+      __syncthreads();
+      for (int64_t b = e0 + tid; b < e1; b += 256) {
+        const float w = logit(row + b);
+        if (w > bound) {
+          const int at = atomicAdd(&count, 1);
+          if (at < LP_CAND) cand[at] = key_of(w, b);
         }
       }
       __syncthreads();
-      n = count[0];
-      for (int64_t b = e0; b < e1 && n < above + k; b += 256) {
+      n = count;
+      search = n > LP_CAND - k;
+      const int want = n + k;
+      for (int64_t b = e0; b < e1 && n < want && !search; b += 256) {
         const bool eq = b + tid < e1 && logit(row + b + tid) == bound;
         const uint64_t bal = __ballot(eq);
         if (lane == 0) red[wave][0] = static_cast<float>(__popcll(bal));
@@ -304,7 +328,7 @@ __global__ void __launch_bounds__(256) logprobs_kernel(LogprobArgs a) {
           if (w < wave) at += cw;
           all += cw;
         }
-        if (eq && at < LP_CAND) cand[at] = ArgBest{bound, static_cast<int32_t>(b + tid)};
+        if (eq && at < LP_CAND) cand[at] = key_of(bound, b + tid);
         n += all;
         __syncthreads();
       }
@@ -312,91 +336,81 @@ __global__ void __launch_bounds__(256) logprobs_kernel(LogprobArgs a) {
     }
   }
   if (search) {
-    const T *row = x + skip;
-    ArgBest last{0.0f, -1};
+    uint64_t last = 0;
     for (int t = 0; t < k; ++t) {
-      ArgBest b{0.0f, -1};
+      uint64_t b = 0;
       for (int64_t q = e0 + tid; q < e1; q += 256) {
-        const ArgBest w{logit(row + q), static_cast<int32_t>(q)};
-        if (t > 0 && !before(last, w)) continue;
-        if (b.i < 0 || before(w, b)) b = w;
+        const uint64_t w = key_of(logit(row + q), q);
+        if ((w < last || t == 0) && w > b) b = w;
       }
       for (int o = 32; o >= 1; o >>= 1) {
-        const ArgBest w{__shfl_xor(b.v, o, 64), __shfl_xor(b.i, o, 64)};
-        if (b.i < 0 || (w.i >= 0 && before(w, b))) b = w;
+        const uint64_t w = __shfl_xor(static_cast<unsigned long long>(b), o, 64);
+        if (w > b) b = w;
       }
       if (lane == 0) bests[wave] = b;
       __syncthreads();
       last = bests[0];
       for (int w = 1; w < 4; ++w)
-        if (last.i < 0 || (bests[w].i >= 0 && before(bests[w], last))) last = bests[w];
+        if (bests[w] > last) last = bests[w];
       __syncthreads();
-      // A slice of fewer columns: entries behind every column.
-      if (last.i < 0) last = ArgBest{-INFINITY, INT32_MAX};
-      if (tid == 0) put(t, last);
+      if (tid == 0) put(t, last);  // 0 behind a slice's last column
     }
     return;
   }
+  if (tid == 0 && (n & 1)) cand[n] = 0;  // n odd: there is room
   __syncthreads();
   for (int i = tid; i < n; i += 256) {
-    const ArgBest b = cand[i];
-    int rank = 0;
-    for (int o = 0; o < n; ++o) rank += cand[o].v > b.v || (cand[o].v == b.v && cand[o].i < b.i) ? 1 : 0;
-    if (rank < k) put(rank, b);
+    const int rank = rank_of(cand, n, cand[i]);
+    if (rank < k) put(rank, cand[i]);
   }
-  for (int i = n + tid; i < k; i += 256) put(i, ArgBest{-INFINITY, INT32_MAX});
+  for (int i = n + tid; i < k; i += 256) put(i, 0);
 }
 
 // Joins the slices of a row.
 template <typename T>
 __global__ void __launch_bounds__(256) logprobs_join_kernel(LogprobArgs a) {
-  __shared__ ArgBest cand[LP_SLICES * MI_TOP_MAX];
+  constexpr int PER = LP_SLICES * MI_TOP_MAX / 256;
+  __shared__ __align__(16) uint64_t cand[LP_SLICES * MI_TOP_MAX];
   __shared__ int count;
   const int tid = threadIdx.x, lane = tid & 63;
   const int64_t r = blockIdx.x;
-  const int ns = a.slices, k = a.top;
+  const int ns = a.slices, k = a.top, all = ns * k;
   const float *st = a.stats + r * ns * 4;
+  const uint64_t *lists = a.lists + r * all;
+  uint64_t mine[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) mine[i] = tid + 256 * i < all ? lists[tid + 256 * i] : 0;
+  // The lists are in order, so where L of them have a q-th key at or above
+  // some key, and L q >= k, the first k are at or above it too: the L-th
+  // largest of the q-th keys bounds what has to be ranked.
+  const int q = k ? (k + ns - 1) / ns : 1, L = (k + q - 1) / q;
+  const uint64_t nth = lane < ns && k ? lists[lane * k + q - 1] : 0;
   const float m = lane < ns ? st[lane * 4] : -FLT_MAX;
   float S = lane < ns ? st[lane * 4 + 1] : 0.0f, Tm = lane < ns ? st[lane * 4 + 2] : 0.0f;
   const float M = fold_max<64>(m);
   rescale(m, M, a.scale * LOG2E, S, Tm);
   S = fold_sum<64>(S);
   Tm = fold_sum<64>(Tm);
-  if (tid == 0) put_stats<T>(a, r, M, S, Tm);
+  if (tid == 0) {
+    put_stats<T>(a, r, M, S, Tm);
+    count = 0;
+  }
   if (k == 0) return;
-  const ArgBest *lists = a.lists + r * ns * k;
-  const int all = ns * k;
-  // A column before the k-th best of the slices' first ones is among the
-  // first k; the others need not be ranked.
-  ArgBest bound{-INFINITY, INT32_MAX};
-  if (ns >= k) {
-    const ArgBest f = lane < ns ? lists[lane * k] : bound;
-    int rank = 0;
-    for (int o = 0; o < ns; ++o) {
-      const ArgBest w{__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f.v), o)),
-                      __builtin_amdgcn_readlane(f.i, o)};
-      rank += before(w, f) ? 1 : 0;
-    }
-    const uint64_t at = __ballot(lane < ns && rank == k - 1);
-    if (at) {
-      const int l = __ffsll(static_cast<unsigned long long>(at)) - 1;
-      bound = ArgBest{__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f.v), l)),
-                      __builtin_amdgcn_readlane(f.i, l)};
-    }
-  }
-  if (tid == 0) count = 0;
+  int above = 0;
+  for (int o = 0; o < ns; ++o) above += lane_key(nth, o) > nth ? 1 : 0;
+  const uint64_t at = __ballot(lane < ns && above == L - 1);
+  const uint64_t bound = at ? lane_key(nth, __ffsll(static_cast<unsigned long long>(at)) - 1) : 0;
   __syncthreads();
-  for (int i = tid; i < all; i += 256) {
-    const ArgBest b = lists[i];
-    if (b.i != INT32_MAX && !before(bound, b)) cand[atomicAdd(&count, 1)] = b;
-  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (mine[i] > 0 && mine[i] >= bound) cand[atomicAdd(&count, 1)] = mine[i];
   __syncthreads();
   const int n = count;
+  if (tid == 0 && (n & 1)) cand[n] = 0;
+  __syncthreads();
   for (int i = tid; i < n; i += 256) {
-    const ArgBest b = cand[i];
-    int rank = 0;
-    for (int o = 0; o < n; ++o) rank += before(cand[o], b) ? 1 : 0;
-    if (rank < k) put_top(a, r * k + rank, b, M, S);
+    const int rank = rank_of(cand, n, cand[i]);
+    if (rank < k) put_top(a, r * k + rank, cand[i], M, S);
   }
 }
 
@@ -430,10 +444,10 @@ int logprobs_run(Ctx *ctx, LogprobArgs a) {
   a.slices = static_cast<int>(ns);
   if (ns > 1) {
     const size_t cells = static_cast<size_t>(a.rows * ns);
-    char *p = static_cast<char *>(scratch(ctx, cells * (16 + sizeof(ArgBest) * a.top)));
+    char *p = static_cast<char *>(scratch(ctx, cells * (16 + sizeof(uint64_t) * a.top)));
     if (!p) return fail(ctx, MI_E_OOM, "token_logprobs scratch");
     a.stats = reinterpret_cast<float *>(p);
-    a.lists = reinterpret_cast<ArgBest *>(p + cells * 16);
+    a.lists = reinterpret_cast<uint64_t *>(p + cells * 16);
   }
   const bool nt = a.rows * a.cols * static_cast<int64_t>(sizeof(T)) >= kStreamBytes;
   const int nl = a.slice <= 256 ? 1 : a.slice <= 512 ? 2 : a.slice <= 1024 ? 4 : C::MAX_NL;
