@@ -190,12 +190,13 @@ typedef float pa_f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int PA_WAVES = 4;
 constexpr int PA_HEADS = 16;       // query heads a block: the matrix cores' tile
-constexpr int PA_UNIT = 64;        // chunk lengths are multiples of it
-constexpr int64_t PA_BLOCKS = 1024;  // blocks the lengths are cut for
+constexpr int PA_UNIT = 128;       // chunk lengths are multiples of it
+constexpr int64_t PA_BLOCKS = 512;   // blocks that run at once: two a CU
+constexpr int64_t PA_CHUNKS = 2048;  // chunks of one sequence at most: the join's weights in LDS
 
-// Positions a wavefront takes a step: 8 KiB of keys.
+// Positions a wavefront takes a step: 8 KiB of keys at most.
 template <int D, typename TC>
-constexpr int pa_pos() { return 8192 / (D * static_cast<int>(sizeof(TC))) > 64 ? 64 : 8192 / (D * static_cast<int>(sizeof(TC))); }
+constexpr int pa_pos() { return D * sizeof(TC) > 256 ? 16 : 32; }
 
 struct AttendArgs {
   const void *q, *k, *v;
@@ -204,8 +205,10 @@ struct AttendArgs {
   PageDiv div;
   int heads, kv_heads, group, tiles, live;  // heads a kv head, their tiles of 16, heads a tile at most
   int q16, out16;
-  int64_t target;  // chunks the lengths are cut for
-  int64_t slots;   // partials there is room for, a kv head tile
+  int32_t least;     // positions a chunk at least
+  double per_chunk;  // 1 / the chunks the lengths are cut for
+  int64_t slots;     // partials there is room for, a kv head tile
+  int2 *cuts;        // a sequence's chunks and the slot of its first partial
   float scale;     // times log2(e)
   float *part;
   void *out;
@@ -236,11 +239,16 @@ __device__ __forceinline__ int32_t pa_len(const AttendArgs &a, int64_t s0, int l
   return static_cast<int32_t>(paged_len(a.lens[s0 + lane], a.per * a.page));
 }
 __device__ __forceinline__ int64_t pa_sum(const AttendArgs &a, int lane, int32_t first) {
-  int64_t t = first;
+  // Halves of 16 bits, whose sums over the lanes hold in 32.
+  int64_t t = lane_value(wave_scan(first & 0xffff), 63) + (static_cast<int64_t>(lane_value(wave_scan(first >> 16), 63)) << 16);
+  if (a.seqs > 64) {
+    int64_t more = 0;
 #pragma unroll 4
-  for (int64_t s0 = 64; s0 < a.seqs; s0 += 64) t += pa_len(a, s0, lane);
+    for (int64_t s0 = 64; s0 < a.seqs; s0 += 64) more += pa_len(a, s0, lane);
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) t += __shfl_xor(t, o, 64);
+    for (int o = 32; o >= 1; o >>= 1) more += __shfl_xor(more, o, 64);
+    t += more;
+  }
   return t;
 }
 
@@ -250,25 +258,17 @@ struct Chunk {
   int64_t seq;
   int32_t c, n, len, slot;
 };
-// Chunk g; or (by_seq) the cut of sequence g.
-template <bool BY_SEQ>
 __device__ __forceinline__ Chunk pa_chunk(const AttendArgs &a, int64_t g, int lane) {
   int32_t len = pa_len(a, 0, lane);
-  const int64_t limit = chunk_limit(pa_sum(a, lane, len), a.target, PA_UNIT);
+  const int64_t limit = chunk_limit(pa_sum(a, lane, len), a.per_chunk, a.least, PA_UNIT);
   int64_t before = 0, slot = 0;
   for (int64_t s0 = 0; s0 < a.seqs; s0 += 64) {
     if (s0) len = pa_len(a, s0, lane);
     const int32_t n = s0 + lane < a.seqs ? chunk_count(len, limit) : 0, cut = n > 1 ? n : 0;
     const int32_t in = wave_scan(n), cuts = wave_scan(cut);
     const int64_t all = lane_value(in, 63);
-    int at = -1;
-    if constexpr (BY_SEQ) {
-      if (g < s0 + 64) at = static_cast<int>(g - s0);
-    } else {
-      if (g < before + all) at = __popcll(__ballot(before + in <= g));
-    }
-    if (at >= 0) {
-      at = __builtin_amdgcn_readfirstlane(at);
+    if (g < before + all) {
+      const int at = __builtin_amdgcn_readfirstlane(__popcll(__ballot(before + in <= g)));
       const int32_t mine = lane_value(n, at);
       Chunk r;
       r.seq = s0 + at;
@@ -485,30 +485,13 @@ __global__ void __launch_bounds__(PA_WAVES * 64) attend_kernel(AttendArgs a) {
   const int parts = a.kv_heads * a.tiles;
   const int64_t g = blockIdx.x / parts;
   const int jt = blockIdx.x % parts, j = jt / a.tiles, h0 = (jt % a.tiles) * PA_HEADS;
-  const Chunk ch = pa_chunk<false>(a, g, lane);
+  const Chunk ch = pa_chunk(a, g, lane);
   if (ch.seq < 0) return;
   const int nh = a.group - h0 < PA_HEADS ? a.group - h0 : PA_HEADS;  // heads of this tile
   const int32_t clen = chunk_len(ch.len, ch.n, PA_UNIT);
   const int64_t from = static_cast<int64_t>(ch.c) * clen;
   const int32_t lo = from < ch.len ? static_cast<int32_t>(from) : ch.len;
   const int32_t hi = ch.len - lo < clen ? ch.len : lo + clen;
-  if (tid == 0 && ch.c == 0 && a.lens[ch.seq] != ch.len) atomicOr(a.flags, FLAG_INDEX_RANGE);
-
-  // Queries, scaled, heads past the tile's as zeros.
-  const int64_t q0 = (ch.seq * a.heads + static_cast<int64_t>(j) * a.group + h0) * D;
-  for (int e = 4 * tid; e < PA_HEADS * D; e += 4 * PA_WAVES * 64) {
-    const int h = e / D, c = e % D;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (h < nh) x = a.q16 ? f32x4_get(static_cast<const uint16_t *>(a.q) + q0 + e) : f32x4_get(static_cast<const float *>(a.q) + q0 + e);
-    *reinterpret_cast<float4 *>(sm + h * QS + c) = make_float4(x.x * a.scale, x.y * a.scale, x.z * a.scale, x.w * a.scale);
-  }
-  __syncthreads();
-
-  W w;
-  w.query(sm, lane);
-#pragma unroll
-  for (int c = 0; c < CP; ++c) w.acc[c] = pa_f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -FLT_MAX, l = 0.0f;
   const TC *K = static_cast<const TC *>(a.k), *V = static_cast<const TC *>(a.v);
   const int32_t *trow = a.table + ch.seq * a.per;
   const int32_t stride = static_cast<int32_t>(a.kv_heads * a.page), jrow = static_cast<int32_t>(j * a.page);
@@ -532,13 +515,44 @@ __global__ void __launch_bounds__(PA_WAVES * 64) attend_kernel(AttendArgs a) {
       rows[b][lane] = id * stride + jrow + (p - static_cast<int32_t>(page_of(static_cast<uint32_t>(p), a.div) * a.page));
     __builtin_amdgcn_wave_barrier();  // read below by this wavefront, whose LDS accesses run in order
   };
-  int32_t i = wave, id = 0;
+  // The first step's page ids and the queries are asked for together, and
+  // the first keys before the queries are waited for.
+  int32_t i = wave, id = 0, id0 = 0;
   int b = 0;
+  if (i < steps) id0 = page_id(i);
+  const int64_t q0 = (ch.seq * a.heads + static_cast<int64_t>(j) * a.group + h0) * D;
+  constexpr int QN = (PA_HEADS * D / 4 + PA_WAVES * 64 - 1) / (PA_WAVES * 64);
+  float4 qv[QN];
+#pragma unroll
+  for (int u = 0; u < QN; ++u) {
+    const int e = 4 * (tid + u * PA_WAVES * 64);
+    qv[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (e < nh * D)
+      qv[u] = a.q16 ? f32x4_get(static_cast<const uint16_t *>(a.q) + q0 + e) : f32x4_get(static_cast<const float *>(a.q) + q0 + e);
+  }
+  W w;
   if (i < steps) {
-    put_rows(i, page_id(i), 0);
     if (i + PA_WAVES < steps) id = page_id(i + PA_WAVES);
+    put_rows(i, id0, 0);
     w.load_k(K, rows[0], lane);
   }
+  // Scaled, heads past the tile's as zeros.
+#pragma unroll
+  for (int u = 0; u < QN; ++u) {
+    const int e = 4 * (tid + u * PA_WAVES * 64);
+    if (e < PA_HEADS * D)
+      *reinterpret_cast<float4 *>(sm + e / D * QS + e % D) =
+          make_float4(qv[u].x * a.scale, qv[u].y * a.scale, qv[u].z * a.scale, qv[u].w * a.scale);
+  }
+  __syncthreads();
+  w.query(sm, lane);
+  if (tid == 0 && ch.c == 0) {
+    if (a.lens[ch.seq] != ch.len) atomicOr(a.flags, FLAG_INDEX_RANGE);
+    if (a.cuts && jt == 0) a.cuts[ch.seq] = make_int2(ch.n, ch.slot);
+  }
+#pragma unroll
+  for (int c = 0; c < CP; ++c) w.acc[c] = pa_f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -FLT_MAX, l = 0.0f;
   for (; i < steps; i += PA_WAVES, b ^= 1) {
     w.load_v(V, rows[b], lane);
     const bool more = i + PA_WAVES < steps;
@@ -629,36 +643,49 @@ __global__ void __launch_bounds__(PA_WAVES * 64) attend_kernel(AttendArgs a) {
 
 // Joins the chunks of a cut sequence, a block a (sequence, query head): the
 // chunks' weights 2^(m_c - M) in LDS, then D / 4 lanes a group, the groups
-// taking the chunks in turn, and the groups' sums added in order.
+// taking the chunks in turn, and the groups' sums added in order.  A thread
+// asks for its first chunks' values together with the statistics.
 template <int D>
 __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a) {
-  constexpr int LP = D / 4, NG = 256 / LP;
+  constexpr int LP = D / 4, NG = 256 / LP, PRE = 4;
   extern __shared__ float wts[];  // a chunk each
   __shared__ float red[4];
   __shared__ float4 sums[256];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t s = blockIdx.x / a.heads;
   const int h = static_cast<int>(blockIdx.x % a.heads);
-  const Chunk ch = pa_chunk<true>(a, s, lane);
-  if (ch.n < 2 || ch.slot + ch.n > a.slots) return;
+  const int2 cut = a.cuts[s];
+  const int n = cut.x;
+  if (n < 2 || cut.y + n > a.slots) return;
   const int j = h / a.group, hg = h % a.group, jt = j * a.tiles + hg / PA_HEADS, ht = hg % PA_HEADS;
   const int64_t parts = a.kv_heads * a.tiles, ps = pa_stride(a.live, D);
-  const float *p = a.part + (static_cast<int64_t>(ch.slot) * parts + jt) * ps;
+  const float *p = a.part + (static_cast<int64_t>(cut.y) * parts + jt) * ps;
   const int64_t step = parts * ps;
-  float M = -INFINITY;
-  for (int c = tid; c < ch.n; c += 256) {
-    const float mc = p[c * step + ht];
-    wts[c] = mc;
-    M = max_nan(M, mc);
+  const int grp = tid / LP, c4 = 4 * (tid % LP);
+  const float *pv = p + pa_acc0(a.live) + ht * D + c4;
+  float4 x[PRE];
+#pragma unroll
+  for (int i = 0; i < PRE; ++i) {
+    const int c = grp + i * NG;
+    x[i] = *reinterpret_cast<const float4 *>(pv + (c < n ? c : n - 1) * step);
   }
+  const int c0 = tid < n ? tid : n - 1;
+  const float m0 = p[c0 * step + ht], l0 = p[c0 * step + a.live + ht];
+  float M = m0;
+  for (int c = tid + 256; c < n; c += 256) M = max_nan(M, p[c * step + ht]);
   M = fold_max<64>(M);
   if (lane == 0) red[wave] = M;
   __syncthreads();
   M = max_nan(max_nan(red[0], red[1]), max_nan(red[2], red[3]));
   __syncthreads();
   float den = 0.0f;
-  for (int c = tid; c < ch.n; c += 256) {
-    const float wt = __builtin_amdgcn_exp2f(wts[c] - M);
+  if (tid < n) {
+    const float wt = __builtin_amdgcn_exp2f(m0 - M);
+    wts[tid] = wt;
+    den = wt * l0;
+  }
+  for (int c = tid + 256; c < n; c += 256) {
+    const float wt = __builtin_amdgcn_exp2f(p[c * step + ht] - M);
     wts[c] = wt;
     den += wt * p[c * step + a.live + ht];
   }
@@ -667,25 +694,25 @@ __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a) {
   __syncthreads();
   den = (red[0] + red[1]) + (red[2] + red[3]);
   den = isnan(den) ? den : (den > FLT_MIN ? den : FLT_MIN);
-  const int grp = tid / LP, c4 = 4 * (tid % LP);
-  const float *pv = p + pa_acc0(a.live) + ht * D + c4;
   float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float wt, float4 y) {
+    t.x += wt * y.x;
+    t.y += wt * y.y;
+    t.z += wt * y.z;
+    t.w += wt * y.w;
+  };
+#pragma unroll
+  for (int i = 0; i < PRE; ++i)
+    if (grp + i * NG < n) add(wts[grp + i * NG], x[i]);
 #pragma unroll 8
-  for (int c = grp; c < ch.n; c += NG) {
-    const float4 x = *reinterpret_cast<const float4 *>(pv + c * step);
-    const float wt = wts[c];
-    t.x += wt * x.x;
-    t.y += wt * x.y;
-    t.z += wt * x.z;
-    t.w += wt * x.w;
-  }
+  for (int c = grp + PRE * NG; c < n; c += NG) add(wts[c], *reinterpret_cast<const float4 *>(pv + c * step));
   sums[tid] = t;
   __syncthreads();
   if (tid < LP) {
     t = sums[tid];
 #pragma unroll
-    for (int x = 1; x < NG; ++x) {
-      const float4 o = sums[x * LP + tid];
+    for (int y = 1; y < NG; ++y) {
+      const float4 o = sums[y * LP + tid];
       t.x += o.x;
       t.y += o.y;
       t.z += o.z;
@@ -701,26 +728,38 @@ __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a) {
 template <int D>
 int attend_launch(Ctx *ctx, AttendArgs a, bool kv16) {
   const int64_t parts = static_cast<int64_t>(a.kv_heads) * a.tiles, cap = a.per * a.page;
-  a.target = PA_BLOCKS / parts > 1 ? PA_BLOCKS / parts : 1;
+  // Chunks for as many rounds of blocks as hold one a sequence twice: a cut
+  // leaves half a chunk a sequence more than the target on average.
+  // Where the sequences alone are many rounds only the longest are cut.
+  const int64_t round = PA_BLOCKS / parts > 1 ? PA_BLOCKS / parts : 1;
+  const int64_t rounds = (2 * a.seqs + round - 1) / round;
+  int64_t target = rounds * round - a.seqs / 2;
+  if (rounds > 8) target = a.seqs / 2 > 6 * round ? a.seqs / 2 : 6 * round;
+  a.least = static_cast<int32_t>((cap + PA_CHUNKS - 1) / PA_CHUNKS);
   // A sequence makes one chunk and at most one more a unit; all of them
   // together at most the target's beside one each.
   const int64_t most = (cap + PA_UNIT - 1) / PA_UNIT;
-  int64_t chunks = a.target + 1 + a.seqs;
+  int64_t chunks = target + a.seqs + 1;
   if (most < chunks / a.seqs) chunks = (most > 1 ? most : 1) * a.seqs;
   const bool cut = most > 1;
-  a.slots = cut ? 2 * a.target + 2 : 0;
+  a.per_chunk = 1.0 / static_cast<double>(target);
+  a.slots = cut ? 2 * target + 2 : 0;
   if (chunks * parts > INT32_MAX || a.seqs * a.heads > INT32_MAX)
     return fail(ctx, MI_E_UNSUPPORTED, "paged_attention: grid too large");
   if (cut) {
-    a.part = static_cast<float *>(scratch(ctx, static_cast<size_t>(a.slots * parts * pa_stride(a.live, D)) * sizeof(float)));
-    if (!a.part) return fail(ctx, MI_E_OOM, "paged_attention scratch");
+    const size_t cuts = (static_cast<size_t>(a.seqs) * sizeof(int2) + 255) / 256 * 256;
+    char *p = static_cast<char *>(scratch(ctx, cuts + static_cast<size_t>(a.slots * parts * pa_stride(a.live, D)) * sizeof(float)));
+    if (!p) return fail(ctx, MI_E_OOM, "paged_attention scratch");
+    a.cuts = reinterpret_cast<int2 *>(p);
+    a.part = reinterpret_cast<float *>(p + cuts);
   }
   const unsigned grid = static_cast<unsigned>(chunks * parts);
   if (kv16) attend_kernel<D, uint16_t><<<grid, PA_WAVES * 64, 0, ctx->stream>>>(a);
   else attend_kernel<D, float><<<grid, PA_WAVES * 64, 0, ctx->stream>>>(a);
   if (int s = check_launch(ctx, "paged_attention")) return s;
   if (!cut) return MI_OK;
-  attend_join_kernel<D><<<static_cast<unsigned>(a.seqs * a.heads), 256, a.slots * sizeof(float), ctx->stream>>>(a);
+  attend_join_kernel<D><<<static_cast<unsigned>(a.seqs * a.heads), 256,
+                          (a.slots < PA_CHUNKS ? a.slots : PA_CHUNKS) * sizeof(float), ctx->stream>>>(a);
   return check_launch(ctx, "paged_attention join");
 }
 

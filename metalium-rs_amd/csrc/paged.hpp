@@ -59,11 +59,14 @@ MI_HD uint32_t page_of(uint32_t n, PageDiv d) {
 // least multiple of `unit` at which all sequences together make about
 // `target` chunks, so every chunk is nearly the same work whatever the
 // lengths; a sequence's chunks are of one length, an idle one has one (empty).
-// target >= 1; sum: the lengths' sum.  Each chunk but a sequence's last is
-// full: a sequence cut in n > 1 has more than (n - 1) C positions, so the
-// chunks of cut sequences are at most 2 sum / C <= 2 target + 2.
-MI_HD int64_t chunk_limit(int64_t sum, int64_t target, int64_t unit) {
-  return (static_cast<int64_t>(static_cast<double>(sum) / static_cast<double>(target)) / unit + 1) * unit;
+// sum: the lengths' sum; per_chunk: 1 / target, target >= 1.  C is above sum /
+// target (to the rounding of a double), so all chunks together are at most
+// target and one a sequence, and those of cut sequences, which hold more than
+// C positions each, at most 2 target.  least: what C is not below (a sequence
+// of up to n least positions makes n chunks at most).
+MI_HD int64_t chunk_limit(int64_t sum, double per_chunk, int64_t least, int64_t unit) {
+  const int64_t c = static_cast<int64_t>(static_cast<double>(sum) * per_chunk);
+  return ((c > least - 1 ? c : least - 1) / unit + 1) * unit;
 }
 MI_HD int32_t chunk_count(int32_t len, int64_t limit) {
   if (len <= limit) return 1;

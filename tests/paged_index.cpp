@@ -12,7 +12,9 @@ int64_t row_of(int64_t p, int64_t j, int64_t o, int64_t kv_heads, int64_t page) 
   return mi::paged_row(p, j, o, kv_heads, page);
 }
 uint32_t quotient(uint32_t n, uint32_t d) { return mi::page_of(n, mi::page_div(d)); }
-int64_t limit_of(int64_t sum, int64_t target, int64_t unit) { return mi::chunk_limit(sum, target, unit); }
+int64_t limit_of(int64_t sum, int64_t target, int64_t least, int64_t unit) {
+  return mi::chunk_limit(sum, 1.0 / static_cast<double>(target), least, unit);
+}
 int32_t count_of(int32_t len, int64_t limit) { return mi::chunk_count(len, limit); }
 int32_t chunk_len_of(int32_t len, int32_t n, int32_t unit) { return mi::chunk_len(len, n, unit); }
 int64_t len_of(int64_t len, int64_t cap) { return mi::paged_len(len, cap); }

@@ -27,7 +27,7 @@ def lib(tmp_path_factory):
     L.row_of.argtypes, L.row_of.restype = [I64] * 5, I64
     U32, I32 = ctypes.c_uint32, ctypes.c_int32
     L.quotient.argtypes, L.quotient.restype = [U32] * 2, U32
-    L.limit_of.argtypes, L.limit_of.restype = [I64] * 3, I64
+    L.limit_of.argtypes, L.limit_of.restype = [I64] * 4, I64
     L.count_of.argtypes = [I32, I64]
     L.chunk_len_of.argtypes = [I32] * 3
     L.len_of.argtypes, L.len_of.restype = [I64] * 2, I64
@@ -92,7 +92,7 @@ def test_quotients(lib):
                 assert lib.quotient(n, d) == n // d, (n, d)
 
 
-@pytest.mark.parametrize("unit", [64])
+@pytest.mark.parametrize("unit", [64, 128])
 def test_chunks_cover_each_sequence_within_bounds(lib, unit):
     rng = random.Random(2)
     cases = [[1], [0], [0] * 70, [64], [65], [I32_MAX], [I32_MAX] * 5, [100000] + [1] * 63, [1] * 3000]
@@ -101,15 +101,16 @@ def test_chunks_cover_each_sequence_within_bounds(lib, unit):
         cases.append([rng.randint(0, hi) for _ in range(rng.randint(1, 80))])
     for lens in cases:
         for target in (1, 7, 128, 1024):
-            limit = lib.limit_of(sum(lens), target, unit)
-            assert limit % unit == 0 and limit >= unit
+            least = -(-max(lens) // 2048)
+            limit = lib.limit_of(sum(lens), target, least, unit)
+            assert limit % unit == 0 and limit >= unit and limit >= least
             chunks = slots = 0
             for n in lens:
                 c = lib.count_of(n, limit)
                 size = lib.chunk_len_of(n, c, unit)
                 assert c >= 1 and (c - 1) * limit <= n <= c * limit
                 assert c * size >= n and (c == 1 or (size % unit == 0 and size <= limit))
-                assert c <= max(1, -(-n // unit))
+                assert c <= max(1, -(-n // unit)) and c <= 2048
                 chunks += c
                 slots += c if c > 1 else 0
             assert chunks <= target + 1 + len(lens)
