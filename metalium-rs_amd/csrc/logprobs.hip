@@ -21,17 +21,17 @@ namespace mi {
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr int LP_CAND = 1024;   // candidates for the alternatives a block holds
-constexpr int LP_TILES = 20;    // tiles a block takes of a row at most
-constexpr int LP_SLICES = 64;   // slices of a row at most: a wavefront's lanes rank them
-constexpr int64_t LP_BLOCKS = 512;  // rows below this are cut in slices
+constexpr int LP_CAND = 1024;         // candidates for the alternatives a block holds
+constexpr int64_t LP_TILE = 512 * 24;  // 16-byte chunks a block takes at most
+constexpr int LP_SLICES = 64;         // slices of a row at most: a wavefront's lanes rank them
+constexpr int64_t LP_BLOCKS = 512;    // rows below this are cut in slices: two blocks a CU
 
 // 16 bytes of a row: 4 F32 or 8 BF16 logits.
 template <typename T>
 struct Chunk16;
 template <>
 struct Chunk16<float> {
-  static constexpr int E = 4, MAX_NL = 8;
+  static constexpr int E = 4;
   template <bool NT>
   static __device__ __forceinline__ uint4 load(const float *p) { return ldu4<NT>(p); }
   static __device__ __forceinline__ float get(const uint4 &v, int e) {
@@ -40,7 +40,7 @@ struct Chunk16<float> {
 };
 template <>
 struct Chunk16<uint16_t> {
-  static constexpr int E = 8, MAX_NL = 4;
+  static constexpr int E = 8;
   template <bool NT>
   static __device__ __forceinline__ uint4 load(const uint16_t *p) { return ldu4<NT>(p); }
   static __device__ __forceinline__ float get(const uint4 &v, int e) {
@@ -109,19 +109,6 @@ __device__ __forceinline__ void rescale(float m, float to, float c, float &S, fl
 // all are -inf, so that those distances are -inf and not NaN.
 __device__ __forceinline__ float origin(float m) { return fmaxf(m, -FLT_MAX); }
 
-// The k-th largest of the lanes' values, equal ones counted as often as they
-// are there.
-__device__ __forceinline__ float kth_largest(float v, int k, int lane) {
-  int rank = 0;
-#pragma unroll 16
-  for (int o = 0; o < 64; ++o) {
-    const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), o));
-    rank += (w > v || (w == v && o < lane)) ? 1 : 0;
-  }
-  const uint64_t at = __ballot(rank == k - 1);
-  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), __ffsll(static_cast<unsigned long long>(at)) - 1));
-}
-
 // A row's results from its statistics over all columns.
 template <typename T>
 __device__ __forceinline__ void put_stats(const LogprobArgs &a, int64_t r, float m, float S, float Tm) {
@@ -142,33 +129,34 @@ __device__ __forceinline__ void put_top(const LogprobArgs &a, int64_t at, uint64
   a.top_ids[at] = key_column(key);
 }
 
-// One slice of a row a block.  Its columns come in tiles of 256 threads x NL
-// chunks of 16 bytes, read once; a thread keeps the sums of its own columns
-// under its own running maximum and joins them with the others' at the end.
+// One slice of a row a block, held in registers: THR threads x NL chunks of 16
+// bytes, all asked for at once and read once (bound by HBM: about ten
+// operations a logit, two of the four bytes' time of an F32 one).  A thread
+// keeps the sums of its own columns under its own running maximum and joins
+// them with the others' at the end.
 //
-// Alternatives: the largest logit of each thread and tile stays in LDS.  The
-// k-th largest of 64 groups' maxima (four threads each) is a bound that at
-// least k columns reach, and only the few cells (thread, tile) that reach it
-// are looked at again -- from registers where the slice is one tile.  The
-// columns found, of the order of k, are ranked against each other.  More equal
-// columns than there is room for (a constant row) are taken in order from the
-// row's start; a row with a NaN or +inf, and one whose columns above the bound
-// are too many, is searched k times.
-template <typename T, int NL, bool TOP, bool NT>
-__global__ void __launch_bounds__(256) logprobs_kernel(LogprobArgs a) {
+// Alternatives: the k-th largest of 64 groups' maxima (THR / 64 threads each)
+// is a bound that at least k columns reach; the few columns that do, of the
+// order of k, are gathered in LDS and ranked against each other.  More columns
+// equal to the bound than there is room for (a constant row) are taken in
+// order from the row's start; a row with a NaN or +inf, and one whose columns
+// above the bound are too many, is searched k times.
+template <typename T, int THR, int NL, bool TOP, bool NT>
+__global__ void __launch_bounds__(THR, THR == 512 ? 4 : 1) logprobs_kernel(LogprobArgs a) {
   using C = Chunk16<T>;
-  constexpr int E = C::E;
-  __shared__ float red[4][3];
+  constexpr int E = C::E, NW = THR / 64;
+  constexpr int STEP = NL < 4 ? NL : NL > 16 ? 2 : 4;  // chunks under one maximum
+  __shared__ float red[NW][3];
   __shared__ float groups[64];
+  __shared__ int ranks[NW][64];
   __shared__ __align__(16) uint64_t cand[TOP ? LP_CAND : 2];
   __shared__ int count;
-  __shared__ uint64_t bests[4];
-  __shared__ float cells[TOP ? LP_TILES : 1][256];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ uint64_t bests[NW];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t r = blockIdx.x / a.slices;
   const int sl = static_cast<int>(blockIdx.x % a.slices);
   // The row from the 16-byte boundary at or before it: column c is element
-  // c + skip.
+  // c + skip there.
   const int64_t flat = r * a.cols;
   const int skip = static_cast<int>(flat & (E - 1));
   const T *x = static_cast<const T *>(a.x) + (flat - skip);
@@ -177,68 +165,68 @@ __global__ void __launch_bounds__(256) logprobs_kernel(LogprobArgs a) {
   const float c = a.scale * LOG2E;
   if (TOP && tid == 0) count = 0;
 
-  uint4 v[NL], nx[NL];
-  auto load = [&](int64_t t0, uint4 (&w)[NL]) {
+  // The slice's chunks from its first, n of them; its columns are elements
+  // lo .. hi - 1 counted from there.
+  const T *base = x + c0 * E;
+  const int n16 = static_cast<int>(c1 - c0);
+  const int lo = c0 == 0 ? skip : 0, hi = c1 == chunks ? static_cast<int>(end - c0 * E) : n16 * E;
+  uint4 v[NL];
 #pragma unroll
-    for (int u = 0; u < NL; ++u) {
-      const int64_t q = t0 + u * 256 + tid;
-      w[u] = C::template load<NT>(x + (q < c1 ? q : c1 - 1) * E);
+  for (int u = 0; u < NL; ++u) {
+    const int q = u * THR + tid;
+    v[u] = C::template load<NT>(base + static_cast<uint32_t>((q < n16 ? q : n16 - 1) * E));
+  }
+  auto mine = [&](int u, int e) {
+    const int i = (u * THR + tid) * E + e;
+    return i >= lo && i < hi;
+  };
+  // A chunk's logits; what lies outside the slice counts as -inf.
+  auto logits = [&](int u, float (&w)[E]) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) w[e] = C::get(v[u], e);
+    if ((u == 0 && lo > 0) || (u + 1) * THR * E > hi) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) w[e] = mine(u, e) ? w[e] : -INFINITY;
     }
   };
-  // Whether element e of the chunk at q is a column of this slice.
-  auto mine = [&](int64_t q, int e) { return q < c1 && q * E + e >= skip && q * E + e < end; };
 
   float mx = -INFINITY, m = -FLT_MAX, S = 0.0f, Tm = 0.0f;
-  int tiles = 0;
-  load(c0, v);
-  for (int64_t t0 = c0; t0 < c1; t0 += 256 * NL, ++tiles) {
-    const bool more = t0 + 256 * NL < c1;
-    if (more) load(t0 + 256 * NL, nx);
-    float xs[NL][E];
+#pragma unroll
+  for (int u0 = 0; u0 < NL; u0 += STEP) {
+    float xs[STEP][E];
     float tm = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < NL; ++u)
-#pragma unroll
-      for (int e = 0; e < E; ++e) xs[u][e] = C::get(v[u], e);
-    if (t0 == 0 || !more) {  // elements outside the slice lie in its ends' tiles
-#pragma unroll
-      for (int u = 0; u < NL; ++u)
-#pragma unroll
-        for (int e = 0; e < E; ++e) xs[u][e] = mine(t0 + u * 256 + tid, e) ? xs[u][e] : -INFINITY;
-    }
-#pragma unroll
-    for (int u = 0; u < NL; ++u)
+    for (int u = 0; u < STEP; ++u) {
+      logits(u0 + u, xs[u]);
 #pragma unroll
       for (int e = 0; e < E; ++e) tm = fmaxf(tm, xs[u][e]);
-    if (TOP) cells[tiles][tid] = tm;
+    }
     if (tm > mx) {
       mx = tm;
       rescale(m, origin(mx), c, S, Tm);
       m = origin(mx);
     }
 #pragma unroll
-    for (int u = 0; u < NL; ++u)
+    for (int u = 0; u < STEP; ++u)
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const float d = (xs[u][e] - m) * c, w = __builtin_amdgcn_exp2f(d);
         S += w;
         Tm = __builtin_fmaf(fmaxf(d, -1e4f), w, Tm);  // 2^-inf = 0 adds nothing
       }
-    if (more) {
-#pragma unroll
-      for (int u = 0; u < NL; ++u) v[u] = nx[u];
-    }
   }
 
   // The block's maximum, then its sums.
   float M = fold_max<64>(mx);
   if (lane == 0) red[wave][0] = M;
   if (TOP) {
-    const float gm = fold_max<4>(mx);
-    if ((lane & 3) == 0) groups[tid >> 2] = gm;
+    const float gm = fold_max<NW>(mx);
+    if ((lane & (NW - 1)) == 0) groups[tid / NW] = gm;
   }
   __syncthreads();
-  M = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
+  M = red[0][0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) M = fmaxf(M, red[w][0]);
   M = origin(M);
   rescale(m, M, c, S, Tm);
   S = fold_sum<64>(S);
@@ -248,8 +236,27 @@ __global__ void __launch_bounds__(256) logprobs_kernel(LogprobArgs a) {
     red[wave][2] = Tm;
   }
   __syncthreads();
-  S = (red[0][1] + red[1][1]) + (red[2][1] + red[3][1]);
-  Tm = (red[0][2] + red[1][2]) + (red[2][2] + red[3][2]);
+  S = red[0][1];
+  Tm = red[0][2];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) {
+    S += red[w][1];
+    Tm += red[w][2];
+  }
+  // How many of the groups' maxima are above each (equal ones in the groups'
+  // order), a wavefront counting over its share of them.
+  float gv = 0.0f;
+  if constexpr (TOP) {
+    gv = groups[lane];
+    int rank = 0;
+#pragma unroll
+    for (int o = 0; o < 64 / NW; ++o) {
+      const int at = wave * (64 / NW) + o;
+      const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(gv), at));
+      rank += w > gv || (w == gv && at < lane) ? 1 : 0;
+    }
+    ranks[wave][lane] = rank;
+  }
   if (tid == 0) {
     if (a.slices == 1) {
       put_stats<T>(a, r, M, S, Tm);
@@ -262,6 +269,7 @@ __global__ void __launch_bounds__(256) logprobs_kernel(LogprobArgs a) {
   }
   if constexpr (!TOP) return;
 
+  __syncthreads();
   const int k = a.top;
   uint64_t *list = a.slices > 1 ? a.lists + (r * a.slices + sl) * k : nullptr;
   auto put = [&](int at, uint64_t key) {
@@ -275,27 +283,45 @@ __global__ void __launch_bounds__(256) logprobs_kernel(LogprobArgs a) {
   int n = 0;
   float bound = -INFINITY;
   if (!search) {
-    bound = kth_largest(groups[lane], k, lane);
-    if (mx >= bound) {
-      for (int t = 0; t < tiles; ++t) {
-        if (!(cells[t][tid] >= bound)) continue;
-        const int64_t t0 = c0 + static_cast<int64_t>(t) * 256 * NL;
-        if (tiles > 1) load(t0, v);
-        uint32_t hits = 0;
+    int rank = 0;
 #pragma unroll
-        for (int u = 0; u < NL; ++u)
+    for (int w = 0; w < NW; ++w) rank += ranks[w][lane];
+    const uint64_t kth = __ballot(rank == k - 1);
+    bound = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(gv), __ffsll(static_cast<unsigned long long>(kth)) - 1));
+    // Two chunks at a time, where any lane's reach the bound.
+    constexpr int G = NL < 2 || NL > 16 ? 1 : 2;
+    const int col0 = static_cast<int>(c0 * E - skip);
+    if (__any(mx >= bound)) {
 #pragma unroll
-          for (int e = 0; e < E; ++e)
-            hits |= (C::get(v[u], e) >= bound && mine(t0 + u * 256 + tid, e) ? 1u : 0u) << (u * E + e);
-        int at = atomicAdd(&count, __popc(hits));
+      for (int u0 = 0; u0 < NL; u0 += G) {
+        float xs[G][E];
+        float tm = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < NL; ++u)
+        for (int u = 0; u < G; ++u) {
+          // The chunk as it was read, not a copy that was made of it above
+          // and kept in registers all along.
+          uint4 &w = v[u0 + u];
+          asm volatile("" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w));
+          logits(u0 + u, xs[u]);
 #pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (hits >> (u * E + e) & 1u) {
-              if (at < LP_CAND) cand[at] = key_of(C::get(v[u], e), (t0 + u * 256 + tid) * E + e - skip);
-              ++at;
-            }
+          for (int e = 0; e < E; ++e) tm = fmaxf(tm, xs[u][e]);
+        }
+        if (tm >= bound) {
+          uint32_t hits = 0;
+#pragma unroll
+          for (int u = 0; u < G; ++u)
+#pragma unroll
+            for (int e = 0; e < E; ++e) hits |= (xs[u][e] >= bound && mine(u0 + u, e) ? 1u : 0u) << (u * E + e);
+          int at = atomicAdd(&count, __popc(hits));
+#pragma unroll
+          for (int u = 0; u < G; ++u)
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+              if (hits >> (u * E + e) & 1u) {
+                if (at < LP_CAND) cand[at] = key_of(xs[u][e], col0 + ((u0 + u) * THR + tid) * E + e);
+                ++at;
+              }
+        }
       }
     }
     __syncthreads();
@@ -306,7 +332,7 @@ __global__ void __launch_bounds__(256) logprobs_kernel(LogprobArgs a) {
       __syncthreads();
       if (tid == 0) count = 0;
       __syncthreads();
-      for (int64_t b = e0 + tid; b < e1; b += 256) {
+      for (int64_t b = e0 + tid; b < e1; b += THR) {
         const float w = logit(row + b);
         if (w > bound) {
           const int at = atomicAdd(&count, 1);
@@ -317,13 +343,13 @@ __global__ void __launch_bounds__(256) logprobs_kernel(LogprobArgs a) {
       n = count;
       search = n > LP_CAND - k;
       const int want = n + k;
-      for (int64_t b = e0; b < e1 && n < want && !search; b += 256) {
+      for (int64_t b = e0; b < e1 && n < want && !search; b += THR) {
         const bool eq = b + tid < e1 && logit(row + b + tid) == bound;
         const uint64_t bal = __ballot(eq);
         if (lane == 0) red[wave][0] = static_cast<float>(__popcll(bal));
         __syncthreads();
         int at = n + __popcll(bal & ((uint64_t(1) << lane) - 1)), all = 0;
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < NW; ++w) {
           const int cw = static_cast<int>(red[w][0]);
           if (w < wave) at += cw;
           all += cw;
@@ -339,7 +365,7 @@ __global__ void __launch_bounds__(256) logprobs_kernel(LogprobArgs a) {
     uint64_t last = 0;
     for (int t = 0; t < k; ++t) {
       uint64_t b = 0;
-      for (int64_t q = e0 + tid; q < e1; q += 256) {
+      for (int64_t q = e0 + tid; q < e1; q += THR) {
         const uint64_t w = key_of(logit(row + q), q);
         if ((w < last || t == 0) && w > b) b = w;
       }
@@ -350,7 +376,7 @@ __global__ void __launch_bounds__(256) logprobs_kernel(LogprobArgs a) {
       if (lane == 0) bests[wave] = b;
       __syncthreads();
       last = bests[0];
-      for (int w = 1; w < 4; ++w)
+      for (int w = 1; w < NW; ++w)
         if (bests[w] > last) last = bests[w];
       __syncthreads();
       if (tid == 0) put(t, last);  // 0 behind a slice's last column
@@ -359,11 +385,11 @@ __global__ void __launch_bounds__(256) logprobs_kernel(LogprobArgs a) {
   }
   if (tid == 0 && (n & 1)) cand[n] = 0;  // n odd: there is room
   __syncthreads();
-  for (int i = tid; i < n; i += 256) {
+  for (int i = tid; i < n; i += THR) {
     const int rank = rank_of(cand, n, cand[i]);
     if (rank < k) put(rank, cand[i]);
   }
-  for (int i = n + tid; i < k; i += 256) put(i, 0);
+  for (int i = n + tid; i < k; i += THR) put(i, 0);
 }
 
 // Joins the slices of a row.
@@ -414,32 +440,34 @@ __global__ void __launch_bounds__(256) logprobs_join_kernel(LogprobArgs a) {
   }
 }
 
-template <typename T, int NL, bool TOP>
+template <typename T, int THR, int NL>
 void logprobs_launch(Ctx *ctx, const LogprobArgs &a, bool nt) {
   const unsigned grid = static_cast<unsigned>(a.rows * a.slices);
-  if (nt) logprobs_kernel<T, NL, TOP, true><<<grid, 256, 0, ctx->stream>>>(a);
-  else logprobs_kernel<T, NL, TOP, false><<<grid, 256, 0, ctx->stream>>>(a);
+  if (a.top > 0) {
+    if (nt) logprobs_kernel<T, THR, NL, true, true><<<grid, THR, 0, ctx->stream>>>(a);
+    else logprobs_kernel<T, THR, NL, true, false><<<grid, THR, 0, ctx->stream>>>(a);
+  } else {
+    if (nt) logprobs_kernel<T, THR, NL, false, true><<<grid, THR, 0, ctx->stream>>>(a);
+    else logprobs_kernel<T, THR, NL, false, false><<<grid, THR, 0, ctx->stream>>>(a);
+  }
 }
 
 template <typename T>
 int logprobs_run(Ctx *ctx, LogprobArgs a) {
-  using C = Chunk16<T>;
-  constexpr int64_t TILE = 256 * C::MAX_NL;
-  const int64_t chunks = (a.cols + 2 * (C::E - 1)) / C::E;  // of a row that starts anywhere
-  int64_t ns = 1;
-  if (a.rows < LP_BLOCKS && chunks > TILE) {
-    const int64_t want = (LP_BLOCKS + a.rows - 1) / a.rows, most = (chunks + 255) / 256;
-    ns = want < most ? want : most;
-    if (ns > LP_SLICES) ns = LP_SLICES;
-  }
-  const int64_t least = (chunks + LP_TILES * TILE - 1) / (LP_TILES * TILE);
-  if (ns < least) ns = least;
+  constexpr int64_t E = Chunk16<T>::E;
+  // Slices of at most a block's registers, and of the fewest that give the
+  // CUs two blocks each while a slice has a chunk for each of 256 threads.
+  const int64_t chunks = a.cols % E ? (a.cols + 2 * (E - 1)) / E : a.cols / E;  // of a row that starts anywhere
+  int64_t ns = (chunks + LP_TILE - 1) / LP_TILE;
+  const int64_t want = (LP_BLOCKS + a.rows - 1) / a.rows, most = chunks / 256;
+  if (ns < want) ns = want < most ? want : (most > ns ? most : ns);
+  if (ns > LP_SLICES) ns = LP_SLICES;
   a.slice = (chunks + ns - 1) / ns;
   // Every slice holds a column of every row: the shortest row's chunks.
-  const int64_t shortest = (a.cols + C::E - 1) / C::E;
+  const int64_t shortest = (a.cols + E - 1) / E;
   ns = (shortest + a.slice - 1) / a.slice;
   if (ns * a.slice < chunks) a.slice = (chunks + ns - 1) / ns;
-  if (ns > LP_SLICES || a.slice > LP_TILES * TILE || a.rows * ns > INT32_MAX)
+  if (a.slice > LP_TILE || a.rows * ns > INT32_MAX)
     return fail(ctx, MI_E_UNSUPPORTED, "token_logprobs of [%lld, %lld]", (long long)a.rows, (long long)a.cols);
   a.slices = static_cast<int>(ns);
   if (ns > 1) {
@@ -450,18 +478,14 @@ int logprobs_run(Ctx *ctx, LogprobArgs a) {
     a.lists = reinterpret_cast<uint64_t *>(p + cells * 16);
   }
   const bool nt = a.rows * a.cols * static_cast<int64_t>(sizeof(T)) >= kStreamBytes;
-  const int nl = a.slice <= 256 ? 1 : a.slice <= 512 ? 2 : a.slice <= 1024 ? 4 : C::MAX_NL;
-  if (a.top > 0) {
-    if (nl == 1) logprobs_launch<T, 1, true>(ctx, a, nt);
-    else if (nl == 2) logprobs_launch<T, 2, true>(ctx, a, nt);
-    else if (nl == 4) logprobs_launch<T, 4, true>(ctx, a, nt);
-    else logprobs_launch<T, C::MAX_NL, true>(ctx, a, nt);
-  } else {
-    if (nl == 1) logprobs_launch<T, 1, false>(ctx, a, nt);
-    else if (nl == 2) logprobs_launch<T, 2, false>(ctx, a, nt);
-    else if (nl == 4) logprobs_launch<T, 4, false>(ctx, a, nt);
-    else logprobs_launch<T, C::MAX_NL, false>(ctx, a, nt);
-  }
+  if (a.slice <= 256) logprobs_launch<T, 256, 1>(ctx, a, nt);
+  else if (a.slice <= 512) logprobs_launch<T, 256, 2>(ctx, a, nt);
+  else if (a.slice <= 1024) logprobs_launch<T, 256, 4>(ctx, a, nt);
+  else if (a.slice <= 2048) logprobs_launch<T, 512, 4>(ctx, a, nt);
+  else if (a.slice <= 4096) logprobs_launch<T, 512, 8>(ctx, a, nt);
+  else if (a.slice <= 6144) logprobs_launch<T, 512, 12>(ctx, a, nt);
+  else if (a.slice <= 8192) logprobs_launch<T, 512, 16>(ctx, a, nt);
+  else logprobs_launch<T, 512, 24>(ctx, a, nt);
   if (int s = check_launch(ctx, "token_logprobs")) return s;
   if (ns == 1) return MI_OK;
   logprobs_join_kernel<T><<<static_cast<unsigned>(a.rows), 256, 0, ctx->stream>>>(a);

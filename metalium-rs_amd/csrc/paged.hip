@@ -309,13 +309,13 @@ __device__ __forceinline__ float head_max(float v) {
 }
 
 // One wavefront's part of a chunk on BF16 pools.
-template <int D>
+template <int D, bool NT>
 struct WaveBf16 {
   static constexpr int POS = pa_pos<D, uint16_t>();
-  static constexpr int NT = POS / 16, KS = D < 32 ? 1 : D / 32, CP = D / 16;  // key steps; columns a lane
+  static constexpr int TILES = POS / 16, KS = D < 32 ? 1 : D / 32, CP = D / 16;  // key steps; columns a lane
   uint4 q[3][KS];
-  uint4 k[NT][KS];
-  uint32_t v[NT][4][CP < 2 ? 1 : CP / 2];
+  uint4 k[TILES][KS];
+  uint32_t v[TILES][4][CP < 2 ? 1 : CP / 2];
   pa_f32x4 acc[CP];
 
   __device__ __forceinline__ void query(const float *qs, int lane) {  // LDS [16][D + 4]
@@ -336,23 +336,23 @@ struct WaveBf16 {
   __device__ __forceinline__ void load_k(const uint16_t *K, const int32_t *rows, int lane) {
     const int g = lane >> 4;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
+    for (int t = 0; t < TILES; ++t) {
       const uint16_t *p = K + static_cast<int64_t>(rows[16 * t + (lane & 15)]) * D + (D < 32 ? 8 * (g & 1) : 8 * g);
 #pragma unroll
-      for (int s = 0; s < KS; ++s) k[t][s] = *reinterpret_cast<const uint4 *>(p + 32 * s);
+      for (int s = 0; s < KS; ++s) k[t][s] = ldu4<NT>(p + 32 * s);
     }
   }
   __device__ __forceinline__ void load_v(const uint16_t *V, const int32_t *rows, int lane) {
     const int n = lane & 15, g = lane >> 4;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
+    for (int t = 0; t < TILES; ++t) {
       const int4 r4 = *reinterpret_cast<const int4 *>(rows + 16 * t + 4 * g);
       const int32_t r[4] = {r4.x, r4.y, r4.z, r4.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint16_t *p = V + static_cast<int64_t>(r[j]) * D + CP * n;
         if constexpr (CP == 8) {
-          const uint4 x = *reinterpret_cast<const uint4 *>(p);
+          const uint4 x = ldu4<NT>(p);
           v[t][j][0] = x.x; v[t][j][1] = x.y; v[t][j][2] = x.z; v[t][j][3] = x.w;
         } else if constexpr (CP == 4) {
           const uint2 x = *reinterpret_cast<const uint2 *>(p);
@@ -377,10 +377,10 @@ struct WaveBf16 {
   }
   // acc += V^T P^T over all tiles, two at a time: contraction step 8 g + j is
   // position 4 g + j % 4 of tile j / 4 of the pair, for both operands.
-  __device__ __forceinline__ void values(const pa_f32x4 (&p)[NT]) {
-    static_assert(NT % 2 == 0, "tiles in pairs");
+  __device__ __forceinline__ void values(const pa_f32x4 (&p)[TILES]) {
+    static_assert(TILES % 2 == 0, "tiles in pairs");
 #pragma unroll
-    for (int t = 0; t < NT; t += 2) {
+    for (int t = 0; t < TILES; t += 2) {
       uint32_t w[3][4];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -402,13 +402,13 @@ struct WaveBf16 {
 
 // The same on F32 pools: 16 x 16 x 4 steps of the F32 matrix cores, whose
 // operand is one value a lane (row or column lane & 15, step lane >> 4).
-template <int D>
+template <int D, bool NT>
 struct WaveF32 {
   static constexpr int POS = pa_pos<D, float>();
-  static constexpr int NT = POS / 16, KQ = D / 16, CP = D / 16;
+  static constexpr int TILES = POS / 16, KQ = D / 16, CP = D / 16;
   float4 q[KQ];
-  float4 k[NT][KQ];
-  float v[NT][4][CP];
+  float4 k[TILES][KQ];
+  float v[TILES][4][CP];
   pa_f32x4 acc[CP];
 
   __device__ __forceinline__ void query(const float *qs, int lane) {
@@ -417,16 +417,16 @@ struct WaveF32 {
   }
   __device__ __forceinline__ void load_k(const float *K, const int32_t *rows, int lane) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
+    for (int t = 0; t < TILES; ++t) {
       const float *p = K + static_cast<int64_t>(rows[16 * t + (lane & 15)]) * D + 4 * (lane >> 4);
 #pragma unroll
-      for (int u = 0; u < KQ; ++u) k[t][u] = *reinterpret_cast<const float4 *>(p + 16 * u);
+      for (int u = 0; u < KQ; ++u) k[t][u] = ld4<NT>(p + 16 * u);
     }
   }
   __device__ __forceinline__ void load_v(const float *V, const int32_t *rows, int lane) {
     const int n = lane & 15, g = lane >> 4;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
+    for (int t = 0; t < TILES; ++t) {
       const int4 r4 = *reinterpret_cast<const int4 *>(rows + 16 * t + 4 * g);
       const int32_t r[4] = {r4.x, r4.y, r4.z, r4.w};
 #pragma unroll
@@ -435,7 +435,7 @@ struct WaveF32 {
         if constexpr (CP >= 4) {
 #pragma unroll
           for (int c = 0; c < CP; c += 4) {
-            const float4 x = *reinterpret_cast<const float4 *>(p + c);
+            const float4 x = ld4<NT>(p + c);
             v[t][j][c] = x.x; v[t][j][c + 1] = x.y; v[t][j][c + 2] = x.z; v[t][j][c + 3] = x.w;
           }
         } else if constexpr (CP == 2) {
@@ -458,9 +458,9 @@ struct WaveF32 {
     }
     return s;
   }
-  __device__ __forceinline__ void values(const pa_f32x4 (&p)[NT]) {
+  __device__ __forceinline__ void values(const pa_f32x4 (&p)[TILES]) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int t = 0; t < TILES; ++t)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -468,15 +468,17 @@ struct WaveF32 {
   }
 };
 
-template <int D, typename TC>
-struct WaveOf { using type = WaveF32<D>; };
-template <int D>
-struct WaveOf<D, uint16_t> { using type = WaveBf16<D>; };
+template <int D, typename TC, bool NT>
+struct WaveOf { using type = WaveF32<D, NT>; };
+template <int D, bool NT>
+struct WaveOf<D, uint16_t, NT> { using type = WaveBf16<D, NT>; };
 
-template <int D, typename TC>
+// NT: the pools are streamed past the caches (they are larger than the last
+// one would keep).
+template <int D, typename TC, bool NT>
 __global__ void __launch_bounds__(PA_WAVES * 64) attend_kernel(AttendArgs a) {
-  using W = typename WaveOf<D, TC>::type;
-  constexpr int POS = W::POS, NT = W::NT, CP = W::CP, QS = D + 4;
+  using W = typename WaveOf<D, TC, NT>::type;
+  constexpr int POS = W::POS, TILES = W::TILES, CP = W::CP, QS = D + 4;
   // The scaled queries, then (once read) the wavefronts' results.
   __shared__ float sm[PA_WAVES * PA_HEADS * QS];
   __shared__ float stat[PA_WAVES][2][PA_HEADS];
@@ -560,21 +562,21 @@ __global__ void __launch_bounds__(PA_WAVES * 64) attend_kernel(AttendArgs a) {
       put_rows(i + PA_WAVES, id, b ^ 1);
       if (i + 2 * PA_WAVES < steps) id = page_id(i + 2 * PA_WAVES);
     }
-    pa_f32x4 s[NT];
+    pa_f32x4 s[TILES];
     float mx = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) s[t] = w.scores(t);
+    for (int t = 0; t < TILES; ++t) s[t] = w.scores(t);
     if (more) w.load_k(K, rows[b ^ 1], lane);
     const int32_t left = hi - lo - i * POS;  // positions from this step's first
     if (left < POS) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < TILES; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (16 * t + 4 * (lane >> 4) + e >= left) s[t][e] = -INFINITY;
     }
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int t = 0; t < TILES; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) mx = max_nan(mx, s[t][e]);
     const float mn = max_nan(m, head_max(mx));
@@ -582,7 +584,7 @@ __global__ void __launch_bounds__(PA_WAVES * 64) attend_kernel(AttendArgs a) {
     m = mn;
     l *= r;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int t = 0; t < TILES; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         s[t][e] = __builtin_amdgcn_exp2f(s[t][e] - mn);
@@ -754,8 +756,12 @@ int attend_launch(Ctx *ctx, AttendArgs a, bool kv16) {
     a.part = reinterpret_cast<float *>(p + cuts);
   }
   const unsigned grid = static_cast<unsigned>(chunks * parts);
-  if (kv16) attend_kernel<D, uint16_t><<<grid, PA_WAVES * 64, 0, ctx->stream>>>(a);
-  else attend_kernel<D, float><<<grid, PA_WAVES * 64, 0, ctx->stream>>>(a);
+  const int64_t pool = 2 * a.pages * a.page * a.kv_heads * D * (kv16 ? 2 : 4);
+  const bool nt = pool >= kStreamBytes;
+  if (kv16 && nt) attend_kernel<D, uint16_t, true><<<grid, PA_WAVES * 64, 0, ctx->stream>>>(a);
+  else if (kv16) attend_kernel<D, uint16_t, false><<<grid, PA_WAVES * 64, 0, ctx->stream>>>(a);
+  else if (nt) attend_kernel<D, float, true><<<grid, PA_WAVES * 64, 0, ctx->stream>>>(a);
+  else attend_kernel<D, float, false><<<grid, PA_WAVES * 64, 0, ctx->stream>>>(a);
   if (int s = check_launch(ctx, "paged_attention")) return s;
   if (!cut) return MI_OK;
   attend_join_kernel<D><<<static_cast<unsigned>(a.seqs * a.heads), 256,
