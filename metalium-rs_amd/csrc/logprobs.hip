@@ -503,94 +503,123 @@ struct LogprobGradArgs {
   uint32_t *flags;
 };
 
-// e^l for l <= 0 or so from the hardware's 2^y, y = l log2(e) rounded: what
-// the rounding and the constant's own leave out (log2(e) = LOG2E + LOG2E_LO)
-// goes into a factor 1 + r, so the error does not grow with |l| (without it
-// 2.2 |l| 2^-24 of the value).
-__device__ __forceinline__ float exp_neg(float l) {
+// e^l for a finite l from the hardware's 2^y, y = l log2(e) rounded: what the
+// rounding and the constant's own leave out (log2(e) = LOG2E + LOG2E_LO) goes
+// into a factor 1 + r, so the error does not grow with |l| (without it 2.2 |l|
+// 2^-24 of the value).
+__device__ __forceinline__ float exp_full(float l) {
   constexpr float LOG2E_LO = 1.925963033500e-8f;
   const float y = l * LOG2E, p = __builtin_amdgcn_exp2f(y);
-  const float r = LN2 * __builtin_fmaf(l, LOG2E_LO, __builtin_fmaf(l, LOG2E, -y));
-  return p == 0.0f ? 0.0f : __builtin_fmaf(p, r, p);
+  return __builtin_fmaf(p, LN2 * __builtin_fmaf(l, LOG2E_LO, __builtin_fmaf(l, LOG2E, -y)), p);
 }
 
-// dx_j = scale (g ([j = target] - p_j) - h p_j (z_j - lse + H)), eight
-// elements a thread and turn, from a 16-byte boundary of both sides at or
-// before the row: one read and one write of each byte, bound by HBM.
-template <typename T, typename TO, bool NT>
+// E consecutive logits widened, and values stored, as 16 bytes of the wider
+// side (8 of a BF16 one beside F32).
+template <int E, bool NT>
+__device__ __forceinline__ void load_logits(const float *p, float (&v)[E]) {
+  const uint4 w = ldu4<NT>(p);
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = Chunk16<float>::get(w, e);
+}
+template <int E, bool NT>
+__device__ __forceinline__ void load_logits(const uint16_t *p, float (&v)[E]) {
+  uint4 w;
+  if constexpr (E == 8) {
+    w = ldu4<NT>(p);
+  } else {
+    const uint2 h = *reinterpret_cast<const uint2 *>(p);
+    w = make_uint4(h.x, h.y, 0, 0);
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = Chunk16<uint16_t>::get(w, e);
+}
+template <int E, bool NT>
+__device__ __forceinline__ void store_grads(float *p, const float (&v)[E]) {
+  st4<NT>(p, make_float4(v[0], v[1], v[2], v[3]));
+}
+template <int E, bool NT>
+__device__ __forceinline__ void store_grads(uint16_t *p, const float (&v)[E]) {
+  if constexpr (E == 8)
+    stu4<NT>(p, make_uint4(bf16x2_bits(v[0], v[1]), bf16x2_bits(v[2], v[3]), bf16x2_bits(v[4], v[5]), bf16x2_bits(v[6], v[7])));
+  else
+    *reinterpret_cast<uint2 *>(p) = make_uint2(bf16x2_bits(v[0], v[1]), bf16x2_bits(v[2], v[3]));
+}
+
+// dx_j = scale (g ([j = target] - p_j) - h p_j (z_j - lse + H)), U chunks of E
+// elements a thread, from a boundary of both sides at or before the row: one
+// read and one write of each byte, bound by HBM.
+template <typename T, typename TO, int U, bool NT>
 __global__ void __launch_bounds__(256) logprobs_backward_kernel(LogprobGradArgs a) {
+  constexpr int E = sizeof(T) == 2 && sizeof(TO) == 2 ? 8 : 4;
   const int64_t r = blockIdx.x / a.blocks;
-  const int blk = static_cast<int>(blockIdx.x % a.blocks);
   const int64_t flat = r * a.cols;
-  const int skip = static_cast<int>(flat & 7);
+  const int skip = static_cast<int>(flat & (E - 1));
   const T *x = static_cast<const T *>(a.x) + (flat - skip);
   TO *o = static_cast<TO *>(a.out) + (flat - skip);
-  const int64_t end = a.cols + skip, chunks = (end + 7) / 8;
+  const int64_t end = a.cols + skip, chunks = (end + E - 1) / E;
+  const int64_t q0 = static_cast<int64_t>(blockIdx.x % a.blocks) * 256 * U + threadIdx.x;
+  float v[U][E];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t q = q0 + u * 256;
+    load_logits<E, NT>(x + (q < chunks ? q : chunks - 1) * E, v[u]);
+  }
   const float lse = a.lse[r], h = a.d_entropy ? a.d_entropy[r] : 0.0f, H = a.d_entropy ? a.entropy[r] : 0.0f;
   float g = a.d_logp ? a.d_logp[r] : 0.0f;
   int64_t target = -1;
   if (a.d_logp) {
     target = a.targets[r];
     if (target < 0 || target >= a.cols) {
-      if (threadIdx.x == 0 && blk == 0) atomicOr(a.flags, FLAG_INDEX_RANGE);
+      if (q0 == 0) atomicOr(a.flags, FLAG_INDEX_RANGE);
       target = -1;
       g = 0.0f;
+    } else {
+      target += skip;
     }
   }
+  // dx_j = scale g [j = target] + p_j (b l_j + c); an empty row has no p.
   const bool none = lse == -INFINITY;
-  if (target >= 0) target += skip;
-  for (int64_t q = static_cast<int64_t>(blk) * 256 + threadIdx.x; q < chunks; q += static_cast<int64_t>(a.blocks) * 256) {
-    float v[8];
-    if constexpr (sizeof(T) == 2) {
-      const uint4 w = ldu4<NT>(x + 8 * q);
+  const float b = none ? 0.0f : -h * a.scale, c = none ? 0.0f : __builtin_fmaf(-g, a.scale, b * H);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = Chunk16<uint16_t>::get(w, e);
-    } else {
-      // The second half of a row's last chunk may lie past the buffer.
-      const bool two = 8 * q + 4 < end;
-      const uint4 w = ldu4<NT>(x + 8 * q), y = ldu4<NT>(x + 8 * q + (two ? 4 : 0));
+  for (int u = 0; u < U; ++u) {
+    const int64_t q = q0 + u * 256;
+    float out[E];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[e] = Chunk16<float>::get(w, e);
-        v[4 + e] = Chunk16<float>::get(y, e);
-      }
+    for (int e = 0; e < E; ++e) {
+      // Where the probability is 0 a finite distance, so that 0 it stays; a
+      // NaN passes.
+      float l = none ? -1e4f : __builtin_fmaf(v[u][e], a.scale, -lse);
+      l = l < -1e4f ? -1e4f : l;
+      out[e] = exp_full(l) * __builtin_fmaf(b, l, c);
     }
-    float out[8];
+    const int64_t t = target - q * E;
+    if (t >= 0 && t < E) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float l = __builtin_fmaf(v[e], a.scale, -lse), p = none ? 0.0f : exp_neg(l);
-      // 0 times a finite bracket where the probability is 0.
-      const float w = p * __builtin_fmaf(h, fmaxf(l, -1e4f) + H, g);
-      out[e] = ((8 * q + e == target ? g : 0.0f) - w) * a.scale;
+      for (int e = 0; e < E; ++e)
+        if (e == t) out[e] = __builtin_fmaf(g, a.scale, out[e]);
     }
-    if (8 * q >= skip && 8 * q + 8 <= end) {
-      if constexpr (sizeof(TO) == 2) {
-        stu4<NT>(o + 8 * q, make_uint4(bf16x2_bits(out[0], out[1]), bf16x2_bits(out[2], out[3]),
-                                       bf16x2_bits(out[4], out[5]), bf16x2_bits(out[6], out[7])));
-      } else {
-        st4<NT>(o + 8 * q, make_float4(out[0], out[1], out[2], out[3]));
-        st4<NT>(o + 8 * q + 4, make_float4(out[4], out[5], out[6], out[7]));
-      }
+    if (q * E >= skip && q * E + E <= end) {
+      store_grads<E, NT>(o + q * E, out);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (8 * q + e >= skip && 8 * q + e < end) f32_put(o + 8 * q + e, out[e]);
+      for (int e = 0; e < E; ++e)
+        if (q * E + e >= skip && q * E + e < end) f32_put(o + q * E + e, out[e]);
     }
   }
 }
 
 template <typename T, typename TO>
 void logprobs_backward_launch(Ctx *ctx, LogprobGradArgs a) {
+  constexpr int64_t E = sizeof(T) == 2 && sizeof(TO) == 2 ? 8 : 4;
   const bool nt = a.rows * a.cols * static_cast<int64_t>(sizeof(T) + sizeof(TO)) >= kStreamBytes;
-  // Four turns a thread, fewer where the rows are few.
-  const int64_t chunks = (a.cols + 14) / 8;
-  int64_t per = (chunks + 1023) / 1024;
-  if (a.rows * per < 1024) per = (1024 + a.rows - 1) / a.rows;
-  const int64_t most = (chunks + 255) / 256;
-  a.blocks = static_cast<int>(per < most ? per : most);
+  const int64_t chunks = (a.cols + 2 * (E - 1)) / E;
+  // Four chunks a thread where that leaves the CUs four blocks each.
+  const bool four = a.rows * ((chunks + 1023) / 1024) >= 1024;
+  a.blocks = static_cast<int>(four ? (chunks + 1023) / 1024 : (chunks + 255) / 256);
   const unsigned grid = static_cast<unsigned>(a.rows * a.blocks);
-  if (nt) logprobs_backward_kernel<T, TO, true><<<grid, 256, 0, ctx->stream>>>(a);
-  else logprobs_backward_kernel<T, TO, false><<<grid, 256, 0, ctx->stream>>>(a);
+  if (four && nt) logprobs_backward_kernel<T, TO, 4, true><<<grid, 256, 0, ctx->stream>>>(a);
+  else if (four) logprobs_backward_kernel<T, TO, 4, false><<<grid, 256, 0, ctx->stream>>>(a);
+  else logprobs_backward_kernel<T, TO, 1, false><<<grid, 256, 0, ctx->stream>>>(a);
 }
 
 int logits_check(Ctx *ctx, const char *what, const Buffer *xb, float scale) {
