@@ -77,52 +77,82 @@ struct AppendArgs {
   int64_t positions;  // rows of the rotary tables
   const int32_t *table, *lens, *starts;
   int64_t rows, seqs, per, pages, page;
-  int heads, kv_heads;
+  PageDiv div, per_row;  // by the page, by a row's items
+  int heads, kv_heads, items, block_rows;
   void *k, *v, *q;
   uint32_t *flags;
 };
 
-// The sequence of row r: the last one whose rows start at or before it --
-// counted over the bounds a wavefront at a time, so a lookup is one or a few
-// independent loads and not a chain of a binary search's.
-__device__ __forceinline__ int64_t append_seq(const AppendArgs &a, int64_t r) {
-  int64_t n = 0;
-  const int lane = threadIdx.x & 63;
-  for (int64_t s0 = 1; s0 <= a.seqs; s0 += 64) {
-    const bool in = s0 + lane <= a.seqs && a.starts[s0 + lane] <= r;
-    n += __popcll(__ballot(in));
-  }
-  return n;
-}
-
-// One new row a block column, eight elements a thread: for a q or k head four
-// of the first half and their partners of the second, for a v head eight in a
-// row.  rope: x cos + rotate(x) sin, two roundings, as mi_rope.
+// Eight elements a thread: for a q or k head four of the first half and their
+// partners of the second, for a v head eight in a row.  A row's items are one
+// or more blocks, or the items of `block_rows` rows share one.  rope: x cos +
+// rotate(x) sin, two roundings, as mi_rope.  Bound by HBM for prompts and by
+// latency for a decode step, so what does not depend on the position -- the
+// row itself -- is asked for before the position is known.  3005 rows of 15
+// heads of 64, F32: X us; 32 rows of 48 heads of 128 into BF16: X us.
 template <typename TI, typename TC, typename TO>
 __global__ void __launch_bounds__(256) append_kernel(AppendArgs a, int D) {
-  const int64_t r = blockIdx.x;
-  const int per_head = D / 8, items = (a.heads + 2 * a.kv_heads) * per_head;
-  const int item = blockIdx.y * 256 + threadIdx.x;
-  int64_t seq = r, first = r, end = r + 1;
-  PagedPos p{PAGED_IDLE, 0};
-  if (a.starts) {
-    seq = append_seq(a, r);
-    if (seq < a.seqs) {
-      first = a.starts[seq];
-      end = a.starts[seq + 1];
-    }
-  }
-  if (seq < a.seqs) p = paged_pos(r, first, end, a.lens[seq], a.per * a.page);
-  int64_t pg = 0;
-  if (p.state == PAGED_OK) {
-    pg = a.table[seq * a.per + p.pos / a.page];
-    if (pg < 0 || pg >= a.pages || p.pos >= a.positions) p.state = PAGED_BAD;
-  }
-  if (p.state == PAGED_BAD && item == 0) atomicOr(a.flags, FLAG_INDEX_RANGE);
-  if (item >= items) return;
-  const int head = item / per_head, quad = item - head * per_head, half = D / 2;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * a.block_rows;
+  const int sub = a.block_rows > 1 ? static_cast<int>(page_of(static_cast<uint32_t>(tid), a.per_row)) : 0;
+  const int item = static_cast<int>(blockIdx.y) * 256 + tid - sub * a.items;
+  const int64_t r = r0 + sub;
+  const bool live = sub < a.block_rows && r < a.rows && item < a.items;
+  const int per_head = D / 8, half = D / 2;
+  const int head = item / per_head, quad = item - head * per_head;
   const bool turn = head < a.heads + a.kv_heads;
   const int c0 = turn ? 4 * quad : 8 * quad, c1 = turn ? c0 + half : c0 + 4;
+  float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
+  if (live) {
+    const TI *x = static_cast<const TI *>(a.qkv) + (r * (a.heads + 2 * a.kv_heads) + head) * D;
+    lo = f32x4_get(x + c0);
+    hi = f32x4_get(x + c1);
+  }
+  // The sequence of a row: behind those whose rows end at or before it,
+  // counted 64 bounds at a time, so a lookup is a few independent loads and
+  // not a chain of a binary search's.
+  int64_t seq = r, first = r, end = r + 1, len = 0;
+  if (a.starts) {
+    seq = a.seqs;
+    int64_t passed = 0;  // the block's rows whose sequence lies behind this batch
+    for (int64_t s0 = 0; s0 < a.seqs && passed < a.block_rows; s0 += 64) {
+      const bool in = s0 + lane < a.seqs;
+      const int32_t from = in ? a.starts[s0 + lane] : 0, to = in ? a.starts[s0 + lane + 1] : INT32_MAX;
+      const int32_t n = in ? a.lens[s0 + lane] : 0;
+      for (int o = static_cast<int>(passed); o < a.block_rows; ++o) {
+        const int at = __popcll(__ballot(to <= r0 + o));
+        if (s0 + at >= a.seqs || at == 64) break;  // rows ascend: the later ones too
+        ++passed;
+        if (sub == o) {
+          seq = s0 + at;
+          first = __builtin_amdgcn_readlane(from, at);
+          end = __builtin_amdgcn_readlane(to, at);
+          len = __builtin_amdgcn_readlane(n, at);
+        }
+      }
+    }
+  } else if (live) {
+    len = a.lens[r];
+  }
+  if (!live) return;
+  PagedPos p{PAGED_IDLE, 0};
+  if (seq < a.seqs) p = paged_pos(r, first, end, len, a.per * a.page);
+  if (p.state == PAGED_OK && p.pos >= a.positions) p.state = PAGED_BAD;
+  int64_t nth = 0, pg = 0;
+  float4 cl = lo, ch = lo, sl = lo, sh = lo;
+  if (p.state == PAGED_OK) {  // the page and the angles in one go
+    nth = page_of(static_cast<uint32_t>(p.pos), a.div);
+    pg = a.table[seq * a.per + nth];
+    if (turn) {
+      const float *cr = a.cosp + p.pos * D, *sr = a.sinp + p.pos * D;
+      cl = f32x4_get(cr + c0);
+      ch = f32x4_get(cr + c1);
+      sl = f32x4_get(sr + c0);
+      sh = f32x4_get(sr + c1);
+    }
+    if (pg < 0 || pg >= a.pages) p.state = PAGED_BAD;
+  }
+  if (p.state == PAGED_BAD && item == 0) atomicOr(a.flags, FLAG_INDEX_RANGE);
   TO *q = static_cast<TO *>(a.q) + (r * a.heads + head) * D;
   if (p.state != PAGED_OK) {
     if (head < a.heads) {
@@ -131,11 +161,7 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a, int D) {
     }
     return;
   }
-  const TI *x = static_cast<const TI *>(a.qkv) + (r * (a.heads + 2 * a.kv_heads) + head) * D;
-  float4 lo = f32x4_get(x + c0), hi = f32x4_get(x + c1);
   if (turn) {
-    const float *cr = a.cosp + p.pos * D, *sr = a.sinp + p.pos * D;
-    const float4 cl = f32x4_get(cr + c0), ch = f32x4_get(cr + c1), sl = f32x4_get(sr + c0), sh = f32x4_get(sr + c1);
     const float4 l = lo, h = hi;
     lo = make_float4(l.x * cl.x + h.x * sl.x, l.y * cl.y + h.y * sl.y, l.z * cl.z + h.z * sl.z, l.w * cl.w + h.w * sl.w);
     hi = make_float4(h.x * ch.x + l.x * sh.x, h.y * ch.y + l.y * sh.y, h.z * ch.z + l.z * sh.z, h.w * ch.w + l.w * sh.w);
@@ -146,15 +172,14 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a, int D) {
     return;
   }
   const int64_t j = turn ? head - a.heads : head - a.heads - a.kv_heads;
-  TC *dst = static_cast<TC *>(turn ? a.k : a.v) + paged_row(pg, j, p.pos % a.page, a.kv_heads, a.page) * D;
+  TC *dst = static_cast<TC *>(turn ? a.k : a.v) + paged_row(pg, j, p.pos - nth * a.page, a.kv_heads, a.page) * D;
   f32x4_put(dst + c0, lo);
   f32x4_put(dst + c1, hi);
 }
 
 template <typename TI, typename TC>
 void append_launch(Ctx *ctx, const AppendArgs &a, int64_t D, int out_elem) {
-  const int64_t items = (a.heads + 2 * static_cast<int64_t>(a.kv_heads)) * (D / 8);
-  const dim3 grid(static_cast<unsigned>(a.rows), grid_for(items, 256));
+  const dim3 grid(static_cast<unsigned>((a.rows + a.block_rows - 1) / a.block_rows), grid_for(a.items, 256));
   if (out_elem == MI_BF16)
     append_kernel<TI, TC, uint16_t><<<grid, 256, 0, ctx->stream>>>(a, static_cast<int>(D));
   else
@@ -828,8 +853,12 @@ extern "C" int mi_qkv_rope_paged(mi_ctx *ctx, mi_id qkv, mi_id cos_table, mi_id 
     a.per = c.per;
     a.pages = c.pages;
     a.page = page;
+    a.div = page_div(static_cast<uint32_t>(page));
     a.heads = static_cast<int>(heads);
     a.kv_heads = static_cast<int>(kv_heads);
+    a.items = static_cast<int>(W / 8);
+    a.per_row = page_div(static_cast<uint32_t>(a.items));
+    a.block_rows = a.items < 256 ? 256 / a.items : 1;
     a.k = c.k;
     a.v = c.v;
     a.q = ob->ptr;
