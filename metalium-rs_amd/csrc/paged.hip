@@ -227,9 +227,9 @@ struct AttendArgs {
   const void *q, *k, *v;
   const int32_t *table, *lens;
   int64_t seqs, per, pages, page;
-  PageDiv div;
+  PageDiv div, by_parts, by_tiles;  // by the page, by the kv heads' tiles, by a kv head's
   int heads, kv_heads, group, tiles, live;  // heads a kv head, their tiles of 16, heads a tile at most
-  int q16, out16;
+  int out16;
   int32_t least;     // positions a chunk at least
   double per_chunk;  // 1 / the chunks the lengths are cut for
   int64_t slots;     // partials there is room for, a kv head tile
@@ -259,9 +259,11 @@ __device__ __forceinline__ int32_t lane_value(int32_t v, int lane) { return __bu
 
 // The lengths of 64 sequences from s0, a lane each (0 past the last), and
 // their sum over all sequences.
-__device__ __forceinline__ int32_t pa_len(const AttendArgs &a, int64_t s0, int lane) {
-  if (s0 + lane >= a.seqs) return 0;
-  return static_cast<int32_t>(paged_len(a.lens[s0 + lane], a.per * a.page));
+__device__ __forceinline__ int32_t pa_len(const AttendArgs &a, int64_t s0, int lane, bool *bad = nullptr) {
+  const int64_t s = s0 + lane < a.seqs ? s0 + lane : a.seqs - 1;
+  const int32_t raw = a.lens[s], len = static_cast<int32_t>(paged_len(raw, a.per * a.page));
+  if (bad) *bad = raw != len;
+  return s0 + lane < a.seqs ? len : 0;
 }
 __device__ __forceinline__ int64_t pa_sum(const AttendArgs &a, int lane, int32_t first) {
   // Halves of 16 bits, whose sums over the lanes hold in 32.
@@ -279,16 +281,18 @@ __device__ __forceinline__ int64_t pa_sum(const AttendArgs &a, int lane, int32_t
 
 // A chunk of the cut: its sequence (-1 past the last chunk), its number of n,
 // the sequence's length, and the slot of the sequence's first partial.
+// Bad: the length was out of range.
 struct Chunk {
   int64_t seq;
-  int32_t c, n, len, slot;
+  int32_t c, n, len, slot, bad;
 };
 __device__ __forceinline__ Chunk pa_chunk(const AttendArgs &a, int64_t g, int lane) {
-  int32_t len = pa_len(a, 0, lane);
+  bool bad;
+  int32_t len = pa_len(a, 0, lane, &bad);
   const int64_t limit = chunk_limit(pa_sum(a, lane, len), a.per_chunk, a.least, PA_UNIT);
   int64_t before = 0, slot = 0;
   for (int64_t s0 = 0; s0 < a.seqs; s0 += 64) {
-    if (s0) len = pa_len(a, s0, lane);
+    if (s0) len = pa_len(a, s0, lane, &bad);
     const int32_t n = s0 + lane < a.seqs ? chunk_count(len, limit) : 0, cut = n > 1 ? n : 0;
     const int32_t in = wave_scan(n), cuts = wave_scan(cut);
     const int64_t all = lane_value(in, 63);
@@ -301,12 +305,13 @@ __device__ __forceinline__ Chunk pa_chunk(const AttendArgs &a, int64_t g, int la
       r.c = static_cast<int32_t>(g - before) - (lane_value(in, at) - mine);
       r.len = lane_value(len, at);
       r.slot = static_cast<int32_t>(slot) + lane_value(cuts, at) - (mine > 1 ? mine : 0);
+      r.bad = static_cast<int32_t>(__ballot(bad) >> at & 1);
       return r;
     }
     before += all;
     slot += lane_value(cuts, 63);
   }
-  return Chunk{-1, 0, 0, 0, 0};
+  return Chunk{-1, 0, 0, 0, 0, 0};
 }
 
 // Three BF16 parts of two F32 values, packed (a in the low halves): each the
@@ -500,18 +505,18 @@ struct WaveOf<D, uint16_t, NT> { using type = WaveBf16<D, NT>; };
 
 // NT: the pools are streamed past the caches (they are larger than the last
 // one would keep).
-template <int D, typename TC, bool NT>
+template <int D, typename TQ, typename TC, bool NT>
 __global__ void __launch_bounds__(PA_WAVES * 64) attend_kernel(AttendArgs a) {
   using W = typename WaveOf<D, TC, NT>::type;
   constexpr int POS = W::POS, TILES = W::TILES, CP = W::CP, QS = D + 4;
   // The scaled queries, then (once read) the wavefronts' results.
   __shared__ float sm[PA_WAVES * PA_HEADS * QS];
   __shared__ float stat[PA_WAVES][2][PA_HEADS];
-  __shared__ __align__(16) int32_t rowbuf[PA_WAVES][2][64];
+  __shared__ __align__(16) int32_t rowbuf[PA_WAVES][2][POS];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int parts = a.kv_heads * a.tiles;
-  const int64_t g = blockIdx.x / parts;
-  const int jt = blockIdx.x % parts, j = jt / a.tiles, h0 = (jt % a.tiles) * PA_HEADS;
+  const int g = static_cast<int>(page_of(blockIdx.x, a.by_parts)), jt = static_cast<int>(blockIdx.x) - g * parts;
+  const int j = static_cast<int>(page_of(static_cast<uint32_t>(jt), a.by_tiles)), h0 = (jt - j * a.tiles) * PA_HEADS;
   const Chunk ch = pa_chunk(a, g, lane);
   if (ch.seq < 0) return;
   const int nh = a.group - h0 < PA_HEADS ? a.group - h0 : PA_HEADS;  // heads of this tile
@@ -519,110 +524,110 @@ __global__ void __launch_bounds__(PA_WAVES * 64) attend_kernel(AttendArgs a) {
   const int64_t from = static_cast<int64_t>(ch.c) * clen;
   const int32_t lo = from < ch.len ? static_cast<int32_t>(from) : ch.len;
   const int32_t hi = ch.len - lo < clen ? ch.len : lo + clen;
-  const TC *K = static_cast<const TC *>(a.k), *V = static_cast<const TC *>(a.v);
-  const int32_t *trow = a.table + ch.seq * a.per;
-  const int32_t stride = static_cast<int32_t>(a.kv_heads * a.page), jrow = static_cast<int32_t>(j * a.page);
-  const int32_t steps = (hi - lo + POS - 1) / POS;
-  int32_t (*rows)[64] = rowbuf[wave];
-  // The pool rows of a step's positions, those past the chunk's end the
-  // last one's again (their scores are dropped below): page ids a step
-  // ahead, so their latency is off the loop.
-  auto position = [&](int32_t i) {
-    const int32_t p = lo + i * POS + (lane & (POS - 1));
-    return p < hi ? p : hi - 1;
-  };
-  auto page_id = [&](int32_t i) { return trow[page_of(static_cast<uint32_t>(position(i)), a.div)]; };
-  auto put_rows = [&](int32_t i, int32_t id, int b) {
-    const int32_t p = position(i);
-    if (id < 0 || id >= a.pages) {
-      atomicOr(a.flags, FLAG_INDEX_RANGE);
-      id = 0;
-    }
-    if (lane < POS)
-      rows[b][lane] = id * stride + jrow + (p - static_cast<int32_t>(page_of(static_cast<uint32_t>(p), a.div) * a.page));
-    __builtin_amdgcn_wave_barrier();  // read below by this wavefront, whose LDS accesses run in order
-  };
-  // The first step's page ids and the queries are asked for together, and
-  // the first keys before the queries are waited for.
-  int32_t i = wave, id = 0, id0 = 0;
-  int b = 0;
-  if (i < steps) id0 = page_id(i);
   const int64_t q0 = (ch.seq * a.heads + static_cast<int64_t>(j) * a.group + h0) * D;
-  constexpr int QN = (PA_HEADS * D / 4 + PA_WAVES * 64 - 1) / (PA_WAVES * 64);
-  float4 qv[QN];
-#pragma unroll
-  for (int u = 0; u < QN; ++u) {
-    const int e = 4 * (tid + u * PA_WAVES * 64);
-    qv[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (e < nh * D)
-      qv[u] = a.q16 ? f32x4_get(static_cast<const uint16_t *>(a.q) + q0 + e) : f32x4_get(static_cast<const float *>(a.q) + q0 + e);
-  }
+
   W w;
-  if (i < steps) {
-    if (i + PA_WAVES < steps) id = page_id(i + PA_WAVES);
-    put_rows(i, id0, 0);
-    w.load_k(K, rows[0], lane);
-  }
-  // Scaled, heads past the tile's as zeros.
-#pragma unroll
-  for (int u = 0; u < QN; ++u) {
-    const int e = 4 * (tid + u * PA_WAVES * 64);
-    if (e < PA_HEADS * D)
-      *reinterpret_cast<float4 *>(sm + e / D * QS + e % D) =
-          make_float4(qv[u].x * a.scale, qv[u].y * a.scale, qv[u].z * a.scale, qv[u].w * a.scale);
-  }
-  __syncthreads();
-  w.query(sm, lane);
-  if (tid == 0 && ch.c == 0) {
-    if (a.lens[ch.seq] != ch.len) atomicOr(a.flags, FLAG_INDEX_RANGE);
-    if (a.cuts && jt == 0) a.cuts[ch.seq] = make_int2(ch.n, ch.slot);
-  }
 #pragma unroll
   for (int c = 0; c < CP; ++c) w.acc[c] = pa_f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -FLT_MAX, l = 0.0f;
-  for (; i < steps; i += PA_WAVES, b ^= 1) {
-    w.load_v(V, rows[b], lane);
-    const bool more = i + PA_WAVES < steps;
-    if (more) {
-      put_rows(i + PA_WAVES, id, b ^ 1);
-      if (i + 2 * PA_WAVES < steps) id = page_id(i + 2 * PA_WAVES);
-    }
-    pa_f32x4 s[TILES];
-    float mx = -INFINITY;
+  bool bad = ch.bad;
+  if (lo < hi) {
+    const TC *K = static_cast<const TC *>(a.k), *V = static_cast<const TC *>(a.v);
+    const int32_t *trow = a.table + ch.seq * a.per;
+    const int32_t stride = static_cast<int32_t>(a.kv_heads * a.page), jrow = static_cast<int32_t>(j * a.page);
+    const int32_t pages = static_cast<int32_t>(a.pages), page = static_cast<int32_t>(a.page);
+    const int32_t steps = (hi - lo + POS - 1) / POS;
+    int32_t (*rows)[POS] = rowbuf[wave];
+    // The pool rows of a step's positions, those past the chunk's end the
+    // last one's again (their scores are dropped below): page ids a step
+    // ahead, so their latency is off the loop.  No load here is under a
+    // condition -- past the last step the last row comes again -- for one
+    // that may or may not be in flight makes every later wait a wait for all.
+    auto position = [&](int32_t i) {  // without a sign: past the end it may pass 2^31
+      const uint32_t p = static_cast<uint32_t>(lo) + static_cast<uint32_t>(i) * POS + (lane & (POS - 1));
+      return p < static_cast<uint32_t>(hi) ? p : static_cast<uint32_t>(hi) - 1;
+    };
+    auto page_id = [&](int32_t i) { return trow[page_of(position(i), a.div)]; };
+    auto put_rows = [&](int32_t i, int32_t id, int b) {
+      const uint32_t p = position(i);
+      const bool out = id < 0 || id >= pages;
+      bad |= out;
+      id = out ? 0 : id;
+      if (lane < POS)
+        rows[b][lane] = id * stride + jrow + static_cast<int32_t>(p - page_of(p, a.div) * static_cast<uint32_t>(page));
+      __builtin_amdgcn_wave_barrier();  // read below by this wavefront, whose LDS accesses run in order
+    };
+    // The first step's page ids and the queries are asked for together, and
+    // the first keys before the queries are waited for; the loop asks for a
+    // step's values at its start and for the next step's keys once its own
+    // are used.
+    int32_t i = wave;
+    int b = 0;
+    const int32_t id0 = page_id(i);
+    constexpr int QN = (PA_HEADS * D / 4 + PA_WAVES * 64 - 1) / (PA_WAVES * 64);
+    float4 qv[QN];
 #pragma unroll
-    for (int t = 0; t < TILES; ++t) s[t] = w.scores(t);
-    if (more) w.load_k(K, rows[b ^ 1], lane);
-    const int32_t left = hi - lo - i * POS;  // positions from this step's first
-    if (left < POS) {
+    for (int u = 0; u < QN; ++u) {
+      const int e = 4 * (tid + u * PA_WAVES * 64);
+      qv[u] = f32x4_get(static_cast<const TQ *>(a.q) + q0 + (e < nh * D ? e : 0));
+    }
+    int32_t id = page_id(i + PA_WAVES);
+    put_rows(i, id0, 0);
+    w.load_k(K, rows[0], lane);
+    // Scaled, heads past the tile's as zeros.
+#pragma unroll
+    for (int u = 0; u < QN; ++u) {
+      const int e = 4 * (tid + u * PA_WAVES * 64);
+      const float f = e < nh * D ? a.scale : 0.0f;
+      float4 x = make_float4(qv[u].x * f, qv[u].y * f, qv[u].z * f, qv[u].w * f);
+      if (e >= nh * D) x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (e < PA_HEADS * D) *reinterpret_cast<float4 *>(sm + e / D * QS + e % D) = x;
+    }
+    __syncthreads();
+    w.query(sm, lane);
+    for (; i < steps; i += PA_WAVES, b ^= 1) {
+      w.load_v(V, rows[b], lane);
+      put_rows(i + PA_WAVES, id, b ^ 1);
+      id = page_id(i + 2 * PA_WAVES);
+      pa_f32x4 s[TILES];
+      float mx = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) s[t] = w.scores(t);
+      w.load_k(K, rows[b ^ 1], lane);
+      const int32_t left = hi - lo - i * POS;  // positions from this step's first
+      if (left < POS) {
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (16 * t + 4 * (lane >> 4) + e >= left) s[t][e] = -INFINITY;
+      }
 #pragma unroll
       for (int t = 0; t < TILES; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (16 * t + 4 * (lane >> 4) + e >= left) s[t][e] = -INFINITY;
+        for (int e = 0; e < 4; ++e) mx = max_nan(mx, s[t][e]);
+      const float mn = max_nan(m, head_max(mx));
+      const float r = __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= r;
+#pragma unroll
+      for (int t = 0; t < TILES; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[t][e] = __builtin_amdgcn_exp2f(s[t][e] - mn);
+          l += s[t][e];
+        }
+#pragma unroll
+      for (int c = 0; c < CP; ++c) w.acc[c] *= r;
+      w.values(s);
     }
-#pragma unroll
-    for (int t = 0; t < TILES; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) mx = max_nan(mx, s[t][e]);
-    const float mn = max_nan(m, head_max(mx));
-    const float r = __builtin_amdgcn_exp2f(m - mn);
-    m = mn;
-    l *= r;
-#pragma unroll
-    for (int t = 0; t < TILES; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[t][e] = __builtin_amdgcn_exp2f(s[t][e] - mn);
-        l += s[t][e];
-      }
-#pragma unroll
-    for (int c = 0; c < CP; ++c) w.acc[c] *= r;
-    w.values(s);
+    __syncthreads();  // the queries are read
   }
+  if (__any(bad) && lane == 0) atomicOr(a.flags, FLAG_INDEX_RANGE);
+  if (tid == 0 && ch.c == 0 && jt == 0 && a.cuts) a.cuts[ch.seq] = make_int2(ch.n, ch.slot);
   l = fold_columns<16>(l);
 
   // The wavefronts' results through LDS: head h's D sums at [wave][h][QS].
-  __syncthreads();
   {
     const int h = lane & 15, gq = lane >> 4;
     if (lane < PA_HEADS) {
@@ -642,28 +647,40 @@ __global__ void __launch_bounds__(PA_WAVES * 64) attend_kernel(AttendArgs a) {
     if (slot >= a.slots) return;  // never: the cut's bound
     part = a.part + (slot * parts + jt) * pa_stride(a.live, D);
   }
-  for (int e = tid; e < nh * D; e += PA_WAVES * 64) {
+  for (int e = 4 * tid; e < nh * D; e += 4 * PA_WAVES * 64) {
     const int h = e / D, c = e % D;
-    float M = stat[0][0][h];
+    float mw[PA_WAVES], lw[PA_WAVES];
+    float4 x[PA_WAVES];
 #pragma unroll
-    for (int x = 1; x < PA_WAVES; ++x) M = max_nan(M, stat[x][0][h]);
-    float sum = 0.0f, den = 0.0f;
+    for (int y = 0; y < PA_WAVES; ++y) {
+      mw[y] = stat[y][0][h];
+      lw[y] = stat[y][1][h];
+      x[y] = *reinterpret_cast<const float4 *>(sm + (y * PA_HEADS + h) * QS + c);
+    }
+    float M = mw[0], den = 0.0f;
 #pragma unroll
-    for (int x = 0; x < PA_WAVES; ++x) {
-      const float wt = __builtin_amdgcn_exp2f(stat[x][0][h] - M);
-      den += wt * stat[x][1][h];
-      sum += wt * sm[(x * PA_HEADS + h) * QS + c];
+    for (int y = 1; y < PA_WAVES; ++y) M = max_nan(M, mw[y]);
+    float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int y = 0; y < PA_WAVES; ++y) {
+      const float wt = __builtin_amdgcn_exp2f(mw[y] - M);
+      den += wt * lw[y];
+      t.x += wt * x[y].x;
+      t.y += wt * x[y].y;
+      t.z += wt * x[y].z;
+      t.w += wt * x[y].w;
     }
     if (part) {
       if (c == 0) {
         part[h] = M;
         part[a.live + h] = den;
       }
-      part[pa_acc0(a.live) + e] = sum;
+      *reinterpret_cast<float4 *>(part + pa_acc0(a.live) + e) = t;
     } else {
       den = isnan(den) ? den : (den > FLT_MIN ? den : FLT_MIN);
-      if (a.out16) f32_put(static_cast<uint16_t *>(a.out) + q0 + e, sum / den);
-      else static_cast<float *>(a.out)[q0 + e] = sum / den;
+      t = make_float4(t.x / den, t.y / den, t.z / den, t.w / den);
+      if (a.out16) f32x4_put(static_cast<uint16_t *>(a.out) + q0 + e, t);
+      else f32x4_put(static_cast<float *>(a.out) + q0 + e, t);
     }
   }
 }
@@ -752,8 +769,17 @@ __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a) {
   }
 }
 
+template <int D, bool NT>
+void attend_types(Ctx *ctx, const AttendArgs &a, unsigned grid, bool q16, bool kv16) {
+  constexpr int THR = PA_WAVES * 64;
+  if (q16 && kv16) attend_kernel<D, uint16_t, uint16_t, NT><<<grid, THR, 0, ctx->stream>>>(a);
+  else if (q16) attend_kernel<D, uint16_t, float, NT><<<grid, THR, 0, ctx->stream>>>(a);
+  else if (kv16) attend_kernel<D, float, uint16_t, NT><<<grid, THR, 0, ctx->stream>>>(a);
+  else attend_kernel<D, float, float, NT><<<grid, THR, 0, ctx->stream>>>(a);
+}
+
 template <int D>
-int attend_launch(Ctx *ctx, AttendArgs a, bool kv16) {
+int attend_launch(Ctx *ctx, AttendArgs a, bool q16, bool kv16) {
   const int64_t parts = static_cast<int64_t>(a.kv_heads) * a.tiles, cap = a.per * a.page;
   // Chunks for as many rounds of blocks as hold one a sequence twice: a cut
   // leaves half a chunk a sequence more than the target on average.
@@ -782,11 +808,8 @@ int attend_launch(Ctx *ctx, AttendArgs a, bool kv16) {
   }
   const unsigned grid = static_cast<unsigned>(chunks * parts);
   const int64_t pool = 2 * a.pages * a.page * a.kv_heads * D * (kv16 ? 2 : 4);
-  const bool nt = pool >= kStreamBytes;
-  if (kv16 && nt) attend_kernel<D, uint16_t, true><<<grid, PA_WAVES * 64, 0, ctx->stream>>>(a);
-  else if (kv16) attend_kernel<D, uint16_t, false><<<grid, PA_WAVES * 64, 0, ctx->stream>>>(a);
-  else if (nt) attend_kernel<D, float, true><<<grid, PA_WAVES * 64, 0, ctx->stream>>>(a);
-  else attend_kernel<D, float, false><<<grid, PA_WAVES * 64, 0, ctx->stream>>>(a);
+  if (pool >= kStreamBytes) attend_types<D, true>(ctx, a, grid, q16, kv16);
+  else attend_types<D, false>(ctx, a, grid, q16, kv16);
   if (int s = check_launch(ctx, "paged_attention")) return s;
   if (!cut) return MI_OK;
   attend_join_kernel<D><<<static_cast<unsigned>(a.seqs * a.heads), 256,
@@ -912,17 +935,18 @@ extern "C" int mi_paged_attention(mi_ctx *ctx, mi_id q, mi_id k_pages, mi_id v_p
     a.group = a.heads / a.kv_heads;
     a.tiles = (a.group + PA_HEADS - 1) / PA_HEADS;
     a.live = a.group < PA_HEADS ? a.group : PA_HEADS;
-    a.q16 = qb->elem == MI_BF16;
+    a.by_parts = page_div(static_cast<uint32_t>(a.kv_heads * a.tiles));
+    a.by_tiles = page_div(static_cast<uint32_t>(a.tiles));
     a.out16 = out_elem == MI_BF16;
     a.scale = scale * 1.4426950408889634f;
     a.out = ob->ptr;
     a.flags = flags(ctx);
-    const bool kv16 = c.elem == MI_BF16;
+    const bool q16 = qb->elem == MI_BF16, kv16 = c.elem == MI_BF16;
     switch (c.D) {
-      case 16: s = attend_launch<16>(ctx, a, kv16); break;
-      case 32: s = attend_launch<32>(ctx, a, kv16); break;
-      case 64: s = attend_launch<64>(ctx, a, kv16); break;
-      default: s = attend_launch<128>(ctx, a, kv16); break;
+      case 16: s = attend_launch<16>(ctx, a, q16, kv16); break;
+      case 32: s = attend_launch<32>(ctx, a, q16, kv16); break;
+      case 64: s = attend_launch<64>(ctx, a, q16, kv16); break;
+      default: s = attend_launch<128>(ctx, a, q16, kv16); break;
     }
     if (s) { mi_free(ctx, id); return s; }
   }
