@@ -8,6 +8,7 @@
 // lie in pages of a shared pool that its row of a page table names, and every
 // sequence has a length of its own, read on the device.
 #include <cfloat>
+#include <type_traits>
 
 #include "common.hpp"
 #include "paged.hpp"
@@ -339,7 +340,7 @@ __device__ __forceinline__ float head_max(float v) {
 }
 
 // One wavefront's part of a chunk on BF16 pools.
-template <int D, bool NT>
+template <int D>
 struct WaveBf16 {
   static constexpr int POS = pa_pos<D, uint16_t>();
   static constexpr int TILES = POS / 16, KS = D < 32 ? 1 : D / 32, CP = D / 16;  // key steps; columns a lane
@@ -363,6 +364,7 @@ struct WaveBf16 {
       for (int p = 0; p < 3; ++p) q[p][t] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
     }
   }
+  template <bool NT>
   __device__ __forceinline__ void load_k(const uint16_t *K, const int32_t *rows, int lane) {
     const int g = lane >> 4;
 #pragma unroll
@@ -372,6 +374,7 @@ struct WaveBf16 {
       for (int s = 0; s < KS; ++s) k[t][s] = ldu4<NT>(p + 32 * s);
     }
   }
+  template <bool NT>
   __device__ __forceinline__ void load_v(const uint16_t *V, const int32_t *rows, int lane) {
     const int n = lane & 15, g = lane >> 4;
 #pragma unroll
@@ -432,7 +435,7 @@ struct WaveBf16 {
 
 // The same on F32 pools: 16 x 16 x 4 steps of the F32 matrix cores, whose
 // operand is one value a lane (row or column lane & 15, step lane >> 4).
-template <int D, bool NT>
+template <int D>
 struct WaveF32 {
   static constexpr int POS = pa_pos<D, float>();
   static constexpr int TILES = POS / 16, KQ = D / 16, CP = D / 16;
@@ -445,6 +448,7 @@ struct WaveF32 {
 #pragma unroll
     for (int u = 0; u < KQ; ++u) q[u] = *reinterpret_cast<const float4 *>(qs + (lane & 15) * (D + 4) + 16 * u + 4 * (lane >> 4));
   }
+  template <bool NT>
   __device__ __forceinline__ void load_k(const float *K, const int32_t *rows, int lane) {
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
@@ -453,6 +457,7 @@ struct WaveF32 {
       for (int u = 0; u < KQ; ++u) k[t][u] = ld4<NT>(p + 16 * u);
     }
   }
+  template <bool NT>
   __device__ __forceinline__ void load_v(const float *V, const int32_t *rows, int lane) {
     const int n = lane & 15, g = lane >> 4;
 #pragma unroll
@@ -498,16 +503,14 @@ struct WaveF32 {
   }
 };
 
-template <int D, typename TC, bool NT>
-struct WaveOf { using type = WaveF32<D, NT>; };
-template <int D, bool NT>
-struct WaveOf<D, uint16_t, NT> { using type = WaveBf16<D, NT>; };
+template <int D, typename TC>
+struct WaveOf { using type = WaveF32<D>; };
+template <int D>
+struct WaveOf<D, uint16_t> { using type = WaveBf16<D>; };
 
-// NT: the pools are streamed past the caches (they are larger than the last
-// one would keep).
-template <int D, typename TQ, typename TC, bool NT>
-__global__ void __launch_bounds__(PA_WAVES * 64) attend_kernel(AttendArgs a) {
-  using W = typename WaveOf<D, TC, NT>::type;
+template <int D, typename TQ, typename TC, bool STREAM>
+__global__ void __launch_bounds__(PA_WAVES * 64, D == 128 ? 2 : 3) attend_kernel(AttendArgs a) {
+  using W = typename WaveOf<D, TC>::type;
   constexpr int POS = W::POS, TILES = W::TILES, CP = W::CP, QS = D + 4;
   // The scaled queries, then (once read) the wavefronts' results.
   __shared__ float sm[PA_WAVES * PA_HEADS * QS];
@@ -564,6 +567,16 @@ __global__ void __launch_bounds__(PA_WAVES * 64) attend_kernel(AttendArgs a) {
     int32_t i = wave;
     int b = 0;
     const int32_t id0 = page_id(i);
+    // STREAM: large pools go past the caches (one sequence of 100001 positions
+    // 72 us, 79 without), unless a neighbouring row of the table begins with
+    // the same page, whose block then reads the same keys (64 rows of one
+    // sequence of 20000: 358 us through the caches, 535 past them).
+    int32_t own = 0, prev = 1, next = 1;
+    if constexpr (STREAM) {
+      own = trow[0];
+      if (ch.seq > 0) prev = a.table[(ch.seq - 1) * a.per];
+      if (ch.seq + 1 < a.seqs) next = a.table[(ch.seq + 1) * a.per];
+    }
     constexpr int QN = (PA_HEADS * D / 4 + PA_WAVES * 64 - 1) / (PA_WAVES * 64);
     float4 qv[QN];
 #pragma unroll
@@ -573,7 +586,13 @@ __global__ void __launch_bounds__(PA_WAVES * 64) attend_kernel(AttendArgs a) {
     }
     int32_t id = page_id(i + PA_WAVES);
     put_rows(i, id0, 0);
-    w.load_k(K, rows[0], lane);
+    bool nt = false;
+    if constexpr (STREAM) {
+      const bool first = ch.seq == 0, last = ch.seq + 1 == a.seqs;
+      nt = !__builtin_amdgcn_readfirstlane((!first && own == prev) || (!last && own == next));
+    }
+    if (STREAM && nt) w.template load_k<true>(K, rows[0], lane);
+    else w.template load_k<false>(K, rows[0], lane);
     // Scaled, heads past the tile's as zeros.
 #pragma unroll
     for (int u = 0; u < QN; ++u) {
@@ -585,42 +604,47 @@ __global__ void __launch_bounds__(PA_WAVES * 64) attend_kernel(AttendArgs a) {
     }
     __syncthreads();
     w.query(sm, lane);
-    for (; i < steps; i += PA_WAVES, b ^= 1) {
-      w.load_v(V, rows[b], lane);
-      put_rows(i + PA_WAVES, id, b ^ 1);
-      id = page_id(i + 2 * PA_WAVES);
-      pa_f32x4 s[TILES];
-      float mx = -INFINITY;
-#pragma unroll
-      for (int t = 0; t < TILES; ++t) s[t] = w.scores(t);
-      w.load_k(K, rows[b ^ 1], lane);
-      const int32_t left = hi - lo - i * POS;  // positions from this step's first
-      if (left < POS) {
-#pragma unroll
-        for (int t = 0; t < TILES; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (16 * t + 4 * (lane >> 4) + e >= left) s[t][e] = -INFINITY;
-      }
-#pragma unroll
-      for (int t = 0; t < TILES; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mx = max_nan(mx, s[t][e]);
-      const float mn = max_nan(m, head_max(mx));
-      const float r = __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      l *= r;
-#pragma unroll
-      for (int t = 0; t < TILES; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[t][e] = __builtin_amdgcn_exp2f(s[t][e] - mn);
-          l += s[t][e];
+    auto run = [&](auto stream) {
+      constexpr bool NT = decltype(stream)::value;
+      for (; i < steps; i += PA_WAVES, b ^= 1) {
+        w.template load_v<NT>(V, rows[b], lane);
+        put_rows(i + PA_WAVES, id, b ^ 1);
+        id = page_id(i + 2 * PA_WAVES);
+        pa_f32x4 s[TILES];
+        float mx = -INFINITY;
+  #pragma unroll
+        for (int t = 0; t < TILES; ++t) s[t] = w.scores(t);
+        w.template load_k<NT>(K, rows[b ^ 1], lane);
+        const int32_t left = hi - lo - i * POS;  // positions from this step's first
+        if (left < POS) {
+  #pragma unroll
+          for (int t = 0; t < TILES; ++t)
+  #pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (16 * t + 4 * (lane >> 4) + e >= left) s[t][e] = -INFINITY;
         }
-#pragma unroll
-      for (int c = 0; c < CP; ++c) w.acc[c] *= r;
-      w.values(s);
-    }
+  #pragma unroll
+        for (int t = 0; t < TILES; ++t)
+  #pragma unroll
+          for (int e = 0; e < 4; ++e) mx = max_nan(mx, s[t][e]);
+        const float mn = max_nan(m, head_max(mx));
+        const float r = __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= r;
+  #pragma unroll
+        for (int t = 0; t < TILES; ++t)
+  #pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[t][e] = __builtin_amdgcn_exp2f(s[t][e] - mn);
+            l += s[t][e];
+          }
+  #pragma unroll
+        for (int c = 0; c < CP; ++c) w.acc[c] *= r;
+        w.values(s);
+      }
+    };
+    if (STREAM && nt) run(std::integral_constant<bool, STREAM>{});
+    else run(std::false_type{});
     __syncthreads();  // the queries are read
   }
   if (__any(bad) && lane == 0) atomicOr(a.flags, FLAG_INDEX_RANGE);
@@ -691,7 +715,7 @@ __global__ void __launch_bounds__(PA_WAVES * 64) attend_kernel(AttendArgs a) {
 // asks for its first chunks' values together with the statistics.
 template <int D>
 __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a) {
-  constexpr int LP = D / 4, NG = 256 / LP, PRE = 4;
+  constexpr int LP = D / 4, NG = 256 / LP, PRE = 8;
   extern __shared__ float wts[];  // a chunk each
   __shared__ float red[4];
   __shared__ float4 sums[256];
@@ -707,14 +731,14 @@ __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a) {
   const int64_t step = parts * ps;
   const int grp = tid / LP, c4 = 4 * (tid % LP);
   const float *pv = p + pa_acc0(a.live) + ht * D + c4;
+  const int c0 = tid < n ? tid : n - 1;
+  const float m0 = p[c0 * step + ht], l0 = p[c0 * step + a.live + ht];
   float4 x[PRE];
 #pragma unroll
   for (int i = 0; i < PRE; ++i) {
     const int c = grp + i * NG;
     x[i] = *reinterpret_cast<const float4 *>(pv + (c < n ? c : n - 1) * step);
   }
-  const int c0 = tid < n ? tid : n - 1;
-  const float m0 = p[c0 * step + ht], l0 = p[c0 * step + a.live + ht];
   float M = m0;
   for (int c = tid + 256; c < n; c += 256) M = max_nan(M, p[c * step + ht]);
   M = fold_max<64>(M);
@@ -769,13 +793,13 @@ __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a) {
   }
 }
 
-template <int D, bool NT>
+template <int D, bool STREAM>
 void attend_types(Ctx *ctx, const AttendArgs &a, unsigned grid, bool q16, bool kv16) {
   constexpr int THR = PA_WAVES * 64;
-  if (q16 && kv16) attend_kernel<D, uint16_t, uint16_t, NT><<<grid, THR, 0, ctx->stream>>>(a);
-  else if (q16) attend_kernel<D, uint16_t, float, NT><<<grid, THR, 0, ctx->stream>>>(a);
-  else if (kv16) attend_kernel<D, float, uint16_t, NT><<<grid, THR, 0, ctx->stream>>>(a);
-  else attend_kernel<D, float, float, NT><<<grid, THR, 0, ctx->stream>>>(a);
+  if (q16 && kv16) attend_kernel<D, uint16_t, uint16_t, STREAM><<<grid, THR, 0, ctx->stream>>>(a);
+  else if (q16) attend_kernel<D, uint16_t, float, STREAM><<<grid, THR, 0, ctx->stream>>>(a);
+  else if (kv16) attend_kernel<D, float, uint16_t, STREAM><<<grid, THR, 0, ctx->stream>>>(a);
+  else attend_kernel<D, float, float, STREAM><<<grid, THR, 0, ctx->stream>>>(a);
 }
 
 template <int D>
@@ -807,8 +831,7 @@ int attend_launch(Ctx *ctx, AttendArgs a, bool q16, bool kv16) {
     a.part = reinterpret_cast<float *>(p + cuts);
   }
   const unsigned grid = static_cast<unsigned>(chunks * parts);
-  const int64_t pool = 2 * a.pages * a.page * a.kv_heads * D * (kv16 ? 2 : 4);
-  if (pool >= kStreamBytes) attend_types<D, true>(ctx, a, grid, q16, kv16);
+  if (2 * a.pages * a.page * a.kv_heads * D * (kv16 ? 2 : 4) >= kStreamBytes) attend_types<D, true>(ctx, a, grid, q16, kv16);
   else attend_types<D, false>(ctx, a, grid, q16, kv16);
   if (int s = check_launch(ctx, "paged_attention")) return s;
   if (!cut) return MI_OK;
