@@ -154,6 +154,19 @@ def test_masked_logits(eng, cols, elem):
     check(eng, x, elem, 1.0, 32, targets=[0, 0, 17, 17, 3])
 
 
+@pytest.mark.parametrize("elem,lanes", [(BF16, 8), (F32, 4)])
+def test_masked_to_a_few_threads_columns(eng, elem, lanes):
+    """What a mask leaves lies in the columns of a few threads, more of them
+    than a block holds as candidates (columns in chunks of `lanes`, a chunk a
+    thread of 512)."""
+    rng = np.random.default_rng(lanes)
+    rows, cols = 512, 2000 * lanes
+    x = rng.standard_normal((rows, cols)).astype(np.float32)
+    x[:, (np.arange(cols) // lanes) % 512 >= 40 * 8 // lanes] = -np.inf
+    x[3:] = x[:1]
+    check(eng, x, elem, 1.0, 32, targets=np.zeros(rows, np.int64))
+
+
 @pytest.mark.parametrize("elem", [F32, BF16])
 @pytest.mark.parametrize("cols", [77, 20000])
 def test_empty_and_not_finite_rows(eng, cols, elem):

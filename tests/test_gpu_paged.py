@@ -320,9 +320,13 @@ def test_attention_types(eng, qe, ce, oe):
 @pytest.mark.parametrize("lens,heads,kv,d,page", [
     ([1], 9, 3, 64, 16), ([577], 9, 3, 64, 16), ([20011], 8, 2, 64, 64), ([9001, 3, 0, 4097], 24, 2, 128, 48),
     ([6000], 4, 4, 32, 6000), ([1] * 300, 4, 1, 16, 16),
+    ([5000] + list(range(200)), 6, 2, 64, 16),
+    (list(range(70)) + [3000, 0, 2500], 4, 2, 16, 8),
+    ([int(17 * i % 90) for i in range(2500)], 2, 1, 16, 16),
 ])
 def test_attention_splits(eng, lens, heads, kv, d, page, ce):
-    """One long sequence, one long among short ones, many short ones."""
+    """One long sequence, one long among short ones, more sequences than a
+    wavefront has lanes, many short ones."""
     rng = np.random.default_rng(len(lens) + d)
     attend_check(eng, Cache(rng, lens, kv, d, page, ce).poison().up(eng), heads)
 
@@ -409,6 +413,37 @@ def test_attention_nan_and_lowest_scores(eng, ce):
         p /= p.sum()
         tol = U * (4 * 72 * (np.abs(k) @ np.abs(qh) * 0.125).max() + 264) * (p @ np.abs(v))
         assert np.all(np.abs(got[2, h] - p @ v) <= tol)
+
+
+@pytest.mark.parametrize("ce", [F32, BF16])
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
+def test_attention_of_large_pools(eng, d, ce):
+    """Pools larger than the last cache, NaN outside the sequences' pages;
+    rows that begin with their neighbour's page and rows that do not."""
+    rng = np.random.default_rng(d)
+    kv, page, lens = 2, 16, [700, 0, 33, 1, 130, 130]
+    small = Cache(rng, lens, kv, d, page, ce)
+    small.table[5] = small.table[4]
+    rows = kv * page
+    pages = (80 << 20) // (rows * d * (4 if ce == F32 else 2))
+    pools = []
+    place = rng.permutation(pages)[:small.pages]
+    for host in (small.k, small.v):
+        src = put(eng, host, ce)[0]
+        pool = eng.fill(pages * rows, d, ce, 0x7FC00000 if ce == F32 else 0x7FC0)
+        for at in range(small.pages):
+            eng.copy_into4(pool, int(place[at]) * rows * d, (0, 0, d, 1), src, at * rows * d, (0, 0, d, 1), (1, 1, rows, d))
+        pools.append(pool)
+    table = np.where((small.table >= 0) & (small.table < small.pages), place[np.clip(small.table, 0, small.pages - 1)], -1)
+    heads, scale = 6, float(np.float32(d ** -0.5))
+    q = rng.standard_normal((len(lens), heads * d)).astype(np.float32)
+    tid, lid = eng.upload_i32(table), eng.upload_i32(np.array(lens).reshape(-1, 1))
+    got = eng.download(eng.paged_attention(eng.upload(q), pools[0], pools[1], tid, lid, heads, kv, page, scale))
+    want, tol = attend64(small, q, heads, scale)
+    assert np.all(np.abs(got.astype(np.float64) - want) <= tol)
+    for p in pools:
+        eng.free(p)
+    eng.sync()
 
 
 def test_attention_past_32_bits(eng):
