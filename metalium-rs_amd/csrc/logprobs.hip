@@ -24,7 +24,8 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int LP_CAND = 1024;         // candidates for the alternatives a block holds
 constexpr int64_t LP_TILE = 512 * 24;  // 16-byte chunks a block takes at most
 constexpr int LP_SLICES = 64;         // slices of a row at most: a wavefront's lanes rank them
-constexpr int64_t LP_BLOCKS = 512;    // rows below this are cut in slices: two blocks a CU
+constexpr int64_t LP_BLOCKS = 512;     // blocks that run at once: two a CU
+constexpr int64_t LP_WHOLE = 65536;    // columns up to which a row is one slice however few the rows
 
 // 16 bytes of a row: 4 F32 or 8 BF16 logits.
 template <typename T>
@@ -455,12 +456,25 @@ void logprobs_launch(Ctx *ctx, const LogprobArgs &a, bool nt) {
 template <typename T>
 int logprobs_run(Ctx *ctx, LogprobArgs a) {
   constexpr int64_t E = Chunk16<T>::E;
-  // Slices of at most a block's registers, and of the fewest that give the
-  // CUs two blocks each while a slice has a chunk for each of 256 threads.
+  // A row is one slice where a block's registers hold it: its results need no
+  // second launch (128 x 49152 BF16, top 20: 13.3 us, 14.9 in 4 slices; 1 x
+  // 49152 F32: 9.6 us, 10.9 in 48).  Wider rows, and few rows of over LP_WHOLE
+  // columns, are cut until the CUs have two blocks each (8 x 128256 BF16: 11.5
+  // us in 63 slices, 19.2 in 2); many wide rows in the number of slices, up to
+  // four times the least, whose last round of blocks is fullest.
   const int64_t chunks = a.cols % E ? (a.cols + 2 * (E - 1)) / E : a.cols / E;  // of a row that starts anywhere
-  int64_t ns = (chunks + LP_TILE - 1) / LP_TILE;
-  const int64_t want = (LP_BLOCKS + a.rows - 1) / a.rows, most = chunks / 256;
-  if (ns < want) ns = want < most ? want : (most > ns ? most : ns);
+  const int64_t least = (chunks + LP_TILE - 1) / LP_TILE, most = chunks / 256;
+  const int64_t want = (LP_BLOCKS + a.rows - 1) / a.rows;
+  int64_t ns = least;
+  if (least > 1 || (a.cols > LP_WHOLE && 2 * a.rows < LP_BLOCKS)) {
+    if (ns < want) ns = want < most ? want : most;
+    if (want <= 4 * least) {
+      auto rounds = [&](int64_t n) { return static_cast<double>((a.rows * n + LP_BLOCKS - 1) / LP_BLOCKS) / static_cast<double>(n); };
+      ns = least;
+      for (int64_t n = least + 1; n <= 4 * least; ++n)
+        if (rounds(n) < 0.95 * rounds(ns)) ns = n;
+    }
+  }
   if (ns > LP_SLICES) ns = LP_SLICES;
   a.slice = (chunks + ns - 1) / ns;
   // Every slice holds a column of every row: the shortest row's chunks.

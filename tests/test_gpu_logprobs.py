@@ -109,7 +109,7 @@ def check(eng, x, elem, scale, top, targets=None, with_targets=True):
 @pytest.mark.parametrize("rows,cols,top", [
     (1, 1, 1), (3, 2, 2), (5, 31, 31), (4, 64, 32), (7, 255, 5), (2, 256, 32), (9, 257, 20), (300, 1000, 5),
     (2, 8192, 32), (3, 8193, 1), (1, 49152, 20), (33, 16385, 8), (2, 40001, 32), (1, 160001, 5), (600, 4099, 3),
-    (1, 500000, 32),
+    (1, 500000, 32), (300, 100001, 7), (20, 70000, 32), (130, 99999, 3), (3, 49152, 32), (1, 12289 * 4, 9),
 ])
 def test_shapes(eng, rows, cols, top, elem):
     rng = np.random.default_rng(rows + cols)
@@ -126,7 +126,7 @@ def test_scales_and_no_targets(eng, scale, elem):
 
 
 @pytest.mark.parametrize("elem", [F32, BF16])
-@pytest.mark.parametrize("cols", [40, 1000, 9001, 50001])
+@pytest.mark.parametrize("cols", [40, 1000, 9001, 50001, 120001])
 def test_ties(eng, cols, elem):
     """Equal logits: the lowest columns, wherever they lie."""
     rng = np.random.default_rng(cols)
@@ -140,7 +140,7 @@ def test_ties(eng, cols, elem):
 
 
 @pytest.mark.parametrize("elem", [F32, BF16])
-@pytest.mark.parametrize("cols", [100, 3001, 50000])
+@pytest.mark.parametrize("cols", [100, 3001, 50000, 120000])
 def test_masked_logits(eng, cols, elem):
     """-inf in all places but some, and values near the type's lowest."""
     rng = np.random.default_rng(cols)
@@ -168,7 +168,7 @@ def test_masked_to_a_few_threads_columns(eng, elem, lanes):
 
 
 @pytest.mark.parametrize("elem", [F32, BF16])
-@pytest.mark.parametrize("cols", [77, 20000])
+@pytest.mark.parametrize("cols", [77, 20000, 100003])
 def test_empty_and_not_finite_rows(eng, cols, elem):
     rng = np.random.default_rng(cols)
     x = rng.standard_normal((5, cols)).astype(np.float32)
@@ -377,7 +377,7 @@ def test_no_rows(eng):
     eng.sync()
 
 
-@pytest.mark.parametrize("rows,cols", [(1, 49152), (40, 5001)])
+@pytest.mark.parametrize("rows,cols", [(1, 49152), (40, 5001), (2, 130001)])
 def test_trace_replays(eng, rows, cols):
     """Forward and backward captured once, replayed on other logits, with an
     eager call of other sizes between: each replay the eager call's bits."""
