@@ -147,6 +147,7 @@ __global__ void __launch_bounds__(THR, THR == 512 ? 4 : 1) logprobs_kernel(Logpr
   using C = Chunk16<T>;
   constexpr int E = C::E, NW = THR / 64;
   constexpr int STEP = NL < 4 ? NL : NL > 16 ? 2 : 4;  // chunks under one maximum
+  constexpr bool KEEP = NL <= 12 || NL * E < 96;       // the chunks' maxima are kept (more would spill)
   __shared__ float red[NW][3];
   __shared__ float groups[64];
   __shared__ int ranks[NW][64];
@@ -192,6 +193,7 @@ __global__ void __launch_bounds__(THR, THR == 512 ? 4 : 1) logprobs_kernel(Logpr
   };
 
   float mx = -INFINITY, m = -FLT_MAX, S = 0.0f, Tm = 0.0f;
+  float cm[KEEP ? NL : 1];
 #pragma unroll
   for (int u0 = 0; u0 < NL; u0 += STEP) {
     float xs[STEP][E];
@@ -199,8 +201,16 @@ __global__ void __launch_bounds__(THR, THR == 512 ? 4 : 1) logprobs_kernel(Logpr
 #pragma unroll
     for (int u = 0; u < STEP; ++u) {
       logits(u0 + u, xs[u]);
+      if constexpr (KEEP) {
+        float um = xs[u][0];
 #pragma unroll
-      for (int e = 0; e < E; ++e) tm = fmaxf(tm, xs[u][e]);
+        for (int e = 1; e < E; ++e) um = fmaxf(um, xs[u][e]);
+        cm[u0 + u] = um;
+        tm = fmaxf(tm, um);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) tm = fmaxf(tm, xs[u][e]);
+      }
     }
     if (tm > mx) {
       mx = tm;
@@ -289,39 +299,33 @@ __global__ void __launch_bounds__(THR, THR == 512 ? 4 : 1) logprobs_kernel(Logpr
     for (int w = 0; w < NW; ++w) rank += ranks[w][lane];
     const uint64_t kth = __ballot(rank == k - 1);
     bound = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(gv), __ffsll(static_cast<unsigned long long>(kth)) - 1));
-    // Two chunks at a time, where any lane's reach the bound.
-    constexpr int G = NL < 2 || NL > 16 ? 1 : 2;
+    // Only the chunks whose largest logit reaches the bound, in any lane.
     const int col0 = static_cast<int>(c0 * E - skip);
     if (__any(mx >= bound)) {
 #pragma unroll
-      for (int u0 = 0; u0 < NL; u0 += G) {
-        float xs[G][E];
-        float tm = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < G; ++u) {
-          // The chunk as it was read, not a copy that was made of it above
-          // and kept in registers all along.
-          uint4 &w = v[u0 + u];
-          asm volatile("" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w));
-          logits(u0 + u, xs[u]);
-#pragma unroll
-          for (int e = 0; e < E; ++e) tm = fmaxf(tm, xs[u][e]);
+      for (int u = 0; u < NL; ++u) {
+        if constexpr (KEEP) {
+          if (!__any(cm[u] >= bound)) continue;
         }
-        if (tm >= bound) {
+        // The chunk as it was read, not a copy that was made of it above and
+        // kept in registers all along.
+        asm volatile("" : "+v"(v[u].x), "+v"(v[u].y), "+v"(v[u].z), "+v"(v[u].w));
+        float xs[E];
+        logits(u, xs);
+        float um = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < E; ++e) um = fmaxf(um, xs[e]);
+        if (um >= bound) {
           uint32_t hits = 0;
 #pragma unroll
-          for (int u = 0; u < G; ++u)
-#pragma unroll
-            for (int e = 0; e < E; ++e) hits |= (xs[u][e] >= bound && mine(u0 + u, e) ? 1u : 0u) << (u * E + e);
+          for (int e = 0; e < E; ++e) hits |= (xs[e] >= bound && mine(u, e) ? 1u : 0u) << e;
           int at = atomicAdd(&count, __popc(hits));
 #pragma unroll
-          for (int u = 0; u < G; ++u)
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-              if (hits >> (u * E + e) & 1u) {
-                if (at < LP_CAND) cand[at] = key_of(xs[u][e], col0 + ((u0 + u) * THR + tid) * E + e);
-                ++at;
-              }
+          for (int e = 0; e < E; ++e)
+            if (hits >> e & 1u) {
+              if (at < LP_CAND) cand[at] = key_of(xs[e], col0 + (u * THR + tid) * E + e);
+              ++at;
+            }
         }
       }
     }
