@@ -147,13 +147,17 @@ __global__ void __launch_bounds__(THR, THR == 512 ? 4 : 1) logprobs_kernel(Logpr
   using C = Chunk16<T>;
   constexpr int E = C::E, NW = THR / 64;
   constexpr int STEP = NL < 4 ? NL : NL > 16 ? 2 : 4;  // chunks under one maximum
-  constexpr bool KEEP = NL <= 12 || NL * E < 96;       // the chunks' maxima are kept (more would spill)
+  // The chunks and their maxima are kept in registers until the bound is
+  // known; more of them would spill: then the maxima wait in LDS and a chunk
+  // that reaches the bound is read again.
+  constexpr bool KEEP = NL <= 12 || NL * E < 96;
   __shared__ float red[NW][3];
   __shared__ float groups[64];
   __shared__ int ranks[NW][64];
   __shared__ __align__(16) uint64_t cand[TOP ? LP_CAND : 2];
   __shared__ int count;
   __shared__ uint64_t bests[NW];
+  __shared__ float maxima[TOP && !KEEP ? NL : 1][THR];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t r = blockIdx.x / a.slices;
   const int sl = static_cast<int>(blockIdx.x % a.slices);
@@ -201,16 +205,12 @@ __global__ void __launch_bounds__(THR, THR == 512 ? 4 : 1) logprobs_kernel(Logpr
 #pragma unroll
     for (int u = 0; u < STEP; ++u) {
       logits(u0 + u, xs[u]);
-      if constexpr (KEEP) {
-        float um = xs[u][0];
+      float um = xs[u][0];
 #pragma unroll
-        for (int e = 1; e < E; ++e) um = fmaxf(um, xs[u][e]);
-        cm[u0 + u] = um;
-        tm = fmaxf(tm, um);
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) tm = fmaxf(tm, xs[u][e]);
-      }
+      for (int e = 1; e < E; ++e) um = fmaxf(um, xs[u][e]);
+      tm = fmaxf(tm, um);
+      if constexpr (KEEP) cm[u0 + u] = um;
+      else if constexpr (TOP) maxima[u0 + u][tid] = um;
     }
     if (tm > mx) {
       mx = tm;
@@ -299,35 +299,52 @@ __global__ void __launch_bounds__(THR, THR == 512 ? 4 : 1) logprobs_kernel(Logpr
     for (int w = 0; w < NW; ++w) rank += ranks[w][lane];
     const uint64_t kth = __ballot(rank == k - 1);
     bound = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(gv), __ffsll(static_cast<unsigned long long>(kth)) - 1));
-    // Only the chunks whose largest logit reaches the bound, in any lane.
+    // Each thread's chunks whose largest logit reaches the bound, one of every
+    // lane a turn: a lane seldom has two, so this is one or two turns of a
+    // short loop (unrolled over the chunks it took 1.4 us a chunk, most of it
+    // for instructions fetched to be run once).
     const int col0 = static_cast<int>(c0 * E - skip);
-    if (__any(mx >= bound)) {
+    uint32_t todo = 0;
+    if (mx >= bound) {
 #pragma unroll
-      for (int u = 0; u < NL; ++u) {
-        if constexpr (KEEP) {
-          if (!__any(cm[u] >= bound)) continue;
+      for (int u = 0; u < NL; ++u) todo |= ((KEEP ? cm[KEEP ? u : 0] : maxima[KEEP ? 0 : u][tid]) >= bound ? 1u : 0u) << u;
+    }
+#pragma nounroll
+    while (__any(todo != 0)) {
+      const int u = todo ? __ffs(todo) - 1 : 0;
+      uint4 w;
+      if constexpr (KEEP) {
+        w = v[0];
+#pragma unroll
+        for (int o = 1; o < NL; ++o) {
+          w.x = u == o ? v[o].x : w.x;
+          w.y = u == o ? v[o].y : w.y;
+          w.z = u == o ? v[o].z : w.z;
+          w.w = u == o ? v[o].w : w.w;
         }
-        // The chunk as it was read, not a copy that was made of it above and
-        // kept in registers all along.
-        asm volatile("" : "+v"(v[u].x), "+v"(v[u].y), "+v"(v[u].z), "+v"(v[u].w));
-        float xs[E];
-        logits(u, xs);
-        float um = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < E; ++e) um = fmaxf(um, xs[e]);
-        if (um >= bound) {
-          uint32_t hits = 0;
-#pragma unroll
-          for (int e = 0; e < E; ++e) hits |= (xs[e] >= bound && mine(u, e) ? 1u : 0u) << e;
-          int at = atomicAdd(&count, __popc(hits));
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (hits >> e & 1u) {
-              if (at < LP_CAND) cand[at] = key_of(xs[e], col0 + (u * THR + tid) * E + e);
-              ++at;
-            }
-        }
+      } else {
+        const int q = u * THR + tid;
+        w = C::template load<false>(base + static_cast<uint32_t>((q < n16 ? q : n16 - 1) * E));
       }
+      uint64_t hit[E];
+      int all = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        hit[e] = __ballot(todo != 0 && C::get(w, e) >= bound && mine(u, e));
+        all += __popcll(hit[e]);
+      }
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&count, all);
+      at = __builtin_amdgcn_readfirstlane(at);
+      const uint64_t below = (uint64_t(1) << lane) - 1;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int mineat = at + __popcll(hit[e] & below);
+        if ((hit[e] >> lane & 1) && mineat < LP_CAND)
+          cand[mineat] = key_of(C::get(w, e), col0 + (u * THR + tid) * E + e);
+        at += __popcll(hit[e]);
+      }
+      todo &= todo - 1;
     }
     __syncthreads();
     n = count;
