@@ -754,11 +754,13 @@ int mi_qkv_rope_paged(mi_ctx *ctx, mi_id qkv, mi_id cos_table, mi_id sin_table,
  * softmax(scale q k^T) v per head with F32 sums (max clamped at -FLT_MAX, sum
  * at FLT_MIN), out [sequences, heads * d] F32, or BF16 rounded once.  An idle
  * sequence gives zeros.  What lies in the pools outside the sequences'
- * positions is not looked at.  Sequences may share pages, and a table row may
- * repeat: several new positions of one sequence are as many rows, each with
- * its own length.  A length outside [0, table columns * page] is read as 0, a
- * page outside the pool as page 0, and either is MI_E_DOMAIN at the next
- * wait. */
+ * positions has no effect on a result.  A NaN key gives NaN in its kv head's
+ * part of the row, a NaN value in its column; an infinite one, or an infinite
+ * query, may give NaN where F32 arithmetic has an infinity.  Sequences may
+ * share pages, and a table row may repeat: several new positions of one
+ * sequence are as many rows, each with its own length.  A length outside
+ * [0, table columns * page] is read as 0, a page outside the pool as page 0,
+ * and either is MI_E_DOMAIN at the next wait. */
 int mi_paged_attention(mi_ctx *ctx, mi_id q, mi_id k_pages, mi_id v_pages,
                        mi_id table, mi_id lens, int64_t heads,
                        int64_t kv_heads, int64_t page, float scale,

@@ -89,8 +89,10 @@ struct AppendArgs {
 // or more blocks, or the items of `block_rows` rows share one.  rope: x cos +
 // rotate(x) sin, two roundings, as mi_rope.  Bound by HBM for prompts and by
 // latency for a decode step, so what does not depend on the position -- the
-// row itself -- is asked for before the position is known.  3005 rows of 15
-// heads of 64, F32: X us; 32 rows of 48 heads of 128 into BF16: X us.
+// row itself -- is asked for before the position is known, and the page and
+// the angles in one go.  3639 rows of 15 heads of 64, F32 (29 MB): 7.3 us, 4.0
+// TB/s; 32 rows of 48 heads of 128 into BF16 pools: 3.0 us, as a launch and
+// two dependent reads take.
 template <typename TI, typename TC, typename TO>
 __global__ void __launch_bounds__(256) append_kernel(AppendArgs a, int D) {
   const int tid = threadIdx.x, lane = tid & 63;
@@ -210,6 +212,12 @@ void append_launch(Ctx *ctx, const AppendArgs &a, int64_t D, int out_elem) {
 // wavefronts take steps of POS positions in turn, each with running maximum
 // and sum, and join in LDS; a chunk of a cut sequence leaves its maximum, sum
 // and sums of values to a second launch that joins them.
+//
+// Measured: one sequence of 100001 positions, 32 heads over 8 of 128, BF16
+// pools (410 MB): 65 us, 6.3 TB/s (a plain streaming read reaches 7.0), and 4.5
+// for the join; 64 sequences of up to 4000: 83 us, 5.7 TB/s, the blocks'
+// unequal ends beside it.  One of 577 positions, 9 heads over 3 of 64, F32: 5.6
+// and 2.8 us, a chain of launch, lengths, table, keys and join, each about 1 us.
 
 typedef __bf16 pa_bf16x8 __attribute__((ext_vector_type(8)));
 typedef float pa_f32x4 __attribute__((ext_vector_type(4)));
