@@ -373,6 +373,9 @@ struct DeviceGuard {
 };
 
 // Grid sizing: blocks to cover `n` items at `per_block`, capped.
+// Threads that one dimension of a launch can hold.
+constexpr int64_t kGridThreads = UINT32_MAX;
+
 inline unsigned grid_for(int64_t n, int64_t per_block, int64_t cap = 1 << 20) {
   int64_t g = (n + per_block - 1) / per_block;
   if (g < 1) g = 1;

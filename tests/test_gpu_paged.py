@@ -331,6 +331,50 @@ def test_attention_splits(eng, lens, heads, kv, d, page, ce):
     attend_check(eng, Cache(rng, lens, kv, d, page, ce).poison().up(eng), heads)
 
 
+@pytest.mark.parametrize("ce", [F32, BF16])
+@pytest.mark.parametrize("seqs,most,heads,kv,d,page", [
+    (63, 700, 4, 2, 32, 16), (64, 1100, 2, 1, 64, 16), (65, 700, 6, 2, 16, 8), (128, 513, 4, 4, 16, 16),
+    (255, 1030, 4, 1, 32, 48), (256, 600, 2, 2, 64, 16), (257, 600, 3, 1, 128, 16), (1024, 520, 2, 1, 16, 8),
+    (1025, 1100, 2, 1, 16, 16), (40, 512, 4, 2, 32, 16), (40, 528, 2, 1, 32, 16), (70, 1024, 4, 2, 32, 16),
+])
+def test_attention_of_cuts_around_their_bounds(eng, seqs, most, heads, kv, d, page, ce):
+    """Sequence counts and table widths on both sides of where the cut of the
+    sequences is formed in another way or left out; empty ones in between."""
+    rng = np.random.default_rng(seqs + most)
+    lens = [int(n) if n % 7 else 0 for n in rng.integers(0, most // 3, seqs)]
+    for at in {0, 1, 3, 4, seqs // 2, seqs - 2, seqs - 1}:
+        lens[at] = most - at % 3
+    attend_check(eng, Cache(rng, lens, kv, d, page, ce).poison().up(eng), heads)
+
+
+@pytest.mark.parametrize("seqs", [64, 200, 300])
+@pytest.mark.parametrize("live", [0, 1, 2])
+def test_attention_of_few_live_sequences_among_many(eng, seqs, live):
+    """All chunks are one sequence's; the idle ones' results are zeros."""
+    rng = np.random.default_rng(seqs + live)
+    lens = [0] * seqs
+    for i in range(live):
+        lens[seqs - 1 - 33 * i] = 2600 - i
+    attend_check(eng, Cache(rng, lens, 2, 32, 16, BF16, width=200).poison().up(eng), 4)
+
+
+@pytest.mark.parametrize("seqs", [70, 300])
+def test_attention_reports_one_bad_length_among_many(eng, seqs):
+    """A length out of range in a lane's second place, and one that only the
+    plan's own launch sees."""
+    rng = np.random.default_rng(seqs)
+    c = Cache(rng, [600] * 2 + [5] * (seqs - 2), 1, 16, 16, F32)
+    c.lens[seqs - 3] = -1
+    c.up(eng)
+    q = eng.upload(rng.standard_normal((seqs, 32)))
+    out = eng.paged_attention(q, c.kid, c.vid, c.tid, c.lid, 2, 1, 16, 0.25)
+    with pytest.raises(miburn.MiError) as e:
+        eng.sync()
+    assert e.value.kind == "DOMAIN"
+    assert not eng.download(out)[seqs - 3].any()
+    eng.sync()
+
+
 def test_attention_no_live_sequence(eng):
     rng = np.random.default_rng(9)
     c = Cache(rng, [0, 0, 0], 2, 64, 16, BF16).poison().up(eng)
