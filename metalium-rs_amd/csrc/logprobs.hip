@@ -507,7 +507,7 @@ int logprobs_run(Ctx *ctx, LogprobArgs a) {
   const int64_t shortest = (a.cols + E - 1) / E;
   ns = (shortest + a.slice - 1) / a.slice;
   if (ns * a.slice < chunks) a.slice = (chunks + ns - 1) / ns;
-  if (a.slice > LP_TILE || a.rows * ns > INT32_MAX)
+  if (a.slice > LP_TILE || a.rows * ns > kGridThreads / 512)
     return fail(ctx, MI_E_UNSUPPORTED, "token_logprobs of [%lld, %lld]", (long long)a.rows, (long long)a.cols);
   a.slices = static_cast<int>(ns);
   if (ns > 1) {
@@ -539,7 +539,8 @@ struct LogprobGradArgs {
   const float *lse, *entropy, *d_logp, *d_entropy;
   float scale;
   void *out;
-  int blocks;  // a row
+  int blocks;    // a row
+  int64_t row0;  // the launch's first
   uint32_t *flags;
 };
 
@@ -585,34 +586,30 @@ __device__ __forceinline__ void store_grads(uint16_t *p, const float (&v)[E]) {
     *reinterpret_cast<uint2 *>(p) = make_uint2(bf16x2_bits(v[0], v[1]), bf16x2_bits(v[2], v[3]));
 }
 
-// dx_j = scale (g ([j = target] - p_j) - h p_j (z_j - lse + H)), U chunks of E
+// dx_j = scale (g ([j = target] - p_j) - h p_j (z_j - lse + H)), a chunk of E
 // elements a thread, from a boundary of both sides at or before the row: one
 // read and one write of each byte, bound by HBM.  2048 x 8192 F32 (134 MB): 23
 // us, 5.8 TB/s; 1001 x 40001 BF16 (160 MB): 29.6 us, 5.4 TB/s; a large copy
 // reaches 5.0.
-template <typename T, typename TO, int U, bool NT>
+template <typename T, typename TO, bool NT>
 __global__ void __launch_bounds__(256) logprobs_backward_kernel(LogprobGradArgs a) {
   constexpr int E = sizeof(T) == 2 && sizeof(TO) == 2 ? 8 : 4;
-  const int64_t r = blockIdx.x / a.blocks;
+  const int64_t r = a.row0 + blockIdx.x / a.blocks;
   const int64_t flat = r * a.cols;
   const int skip = static_cast<int>(flat & (E - 1));
   const T *x = static_cast<const T *>(a.x) + (flat - skip);
   TO *o = static_cast<TO *>(a.out) + (flat - skip);
   const int64_t end = a.cols + skip, chunks = (end + E - 1) / E;
-  const int64_t q0 = static_cast<int64_t>(blockIdx.x % a.blocks) * 256 * U + threadIdx.x;
-  float v[U][E];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int64_t q = q0 + u * 256;
-    load_logits<E, NT>(x + (q < chunks ? q : chunks - 1) * E, v[u]);
-  }
+  const int64_t q = static_cast<int64_t>(blockIdx.x % a.blocks) * 256 + threadIdx.x;
+  float v[E];
+  load_logits<E, NT>(x + (q < chunks ? q : chunks - 1) * E, v);
   const float lse = a.lse[r], h = a.d_entropy ? a.d_entropy[r] : 0.0f, H = a.d_entropy ? a.entropy[r] : 0.0f;
   float g = a.d_logp ? a.d_logp[r] : 0.0f;
   int64_t target = -1;
   if (a.d_logp) {
     target = a.targets[r];
     if (target < 0 || target >= a.cols) {
-      if (q0 == 0) atomicOr(a.flags, FLAG_INDEX_RANGE);
+      if (q == 0) atomicOr(a.flags, FLAG_INDEX_RANGE);
       target = -1;
       g = 0.0f;
     } else {
@@ -622,31 +619,27 @@ __global__ void __launch_bounds__(256) logprobs_backward_kernel(LogprobGradArgs 
   // dx_j = scale g [j = target] + p_j (b l_j + c); an empty row has no p.
   const bool none = lse == -INFINITY;
   const float b = none ? 0.0f : -h * a.scale, c = none ? 0.0f : __builtin_fmaf(-g, a.scale, b * H);
+  float out[E];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int64_t q = q0 + u * 256;
-    float out[E];
+  for (int e = 0; e < E; ++e) {
+    // Where the probability is 0 a finite distance, so that 0 it stays; a
+    // NaN passes.
+    float l = none ? -1e4f : __builtin_fmaf(v[e], a.scale, -lse);
+    l = l < -1e4f ? -1e4f : l;
+    out[e] = exp_full(l) * __builtin_fmaf(b, l, c);
+  }
+  const int64_t t = target - q * E;
+  if (t >= 0 && t < E) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      // Where the probability is 0 a finite distance, so that 0 it stays; a
-      // NaN passes.
-      float l = none ? -1e4f : __builtin_fmaf(v[u][e], a.scale, -lse);
-      l = l < -1e4f ? -1e4f : l;
-      out[e] = exp_full(l) * __builtin_fmaf(b, l, c);
-    }
-    const int64_t t = target - q * E;
-    if (t >= 0 && t < E) {
+    for (int e = 0; e < E; ++e)
+      if (e == t) out[e] = __builtin_fmaf(g, a.scale, out[e]);
+  }
+  if (q * E >= skip && q * E + E <= end) {
+    store_grads<E, NT>(o + q * E, out);
+  } else {
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (e == t) out[e] = __builtin_fmaf(g, a.scale, out[e]);
-    }
-    if (q * E >= skip && q * E + E <= end) {
-      store_grads<E, NT>(o + q * E, out);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (q * E + e >= skip && q * E + e < end) f32_put(o + q * E + e, out[e]);
-    }
+    for (int e = 0; e < E; ++e)
+      if (q * E + e >= skip && q * E + e < end) f32_put(o + q * E + e, out[e]);
   }
 }
 
@@ -655,13 +648,17 @@ void logprobs_backward_launch(Ctx *ctx, LogprobGradArgs a) {
   constexpr int64_t E = sizeof(T) == 2 && sizeof(TO) == 2 ? 8 : 4;
   const bool nt = a.rows * a.cols * static_cast<int64_t>(sizeof(T) + sizeof(TO)) >= kStreamBytes;
   const int64_t chunks = (a.cols + 2 * (E - 1)) / E;
-  // Four chunks a thread where that leaves the CUs four blocks each.
-  const bool four = a.rows * ((chunks + 1023) / 1024) >= 1024;
-  a.blocks = static_cast<int>(four ? (chunks + 1023) / 1024 : (chunks + 255) / 256);
-  const unsigned grid = static_cast<unsigned>(a.rows * a.blocks);
-  if (four && nt) logprobs_backward_kernel<T, TO, 4, true><<<grid, 256, 0, ctx->stream>>>(a);
-  else if (four) logprobs_backward_kernel<T, TO, 4, false><<<grid, 256, 0, ctx->stream>>>(a);
-  else logprobs_backward_kernel<T, TO, 1, false><<<grid, 256, 0, ctx->stream>>>(a);
+  // Four a thread: 8.7 us where one takes 7.2 (512 x 8192 F32), 8.8 and 8.1
+  // (256 x 32000 BF16), 25.3 and 23.3 (2048 x 8192 F32), 32.5 and 33.7 (1001 x
+  // 40001 BF16).
+  a.blocks = static_cast<int>((chunks + 255) / 256);
+  // All rows in one launch, but for more blocks than one can have.
+  const int64_t span = std::max<int64_t>(kGridThreads / 256 / a.blocks, 1);
+  for (a.row0 = 0; a.row0 < a.rows; a.row0 += span) {
+    const unsigned grid = static_cast<unsigned>(std::min(span, a.rows - a.row0) * a.blocks);
+    if (nt) logprobs_backward_kernel<T, TO, true><<<grid, 256, 0, ctx->stream>>>(a);
+    else logprobs_backward_kernel<T, TO, false><<<grid, 256, 0, ctx->stream>>>(a);
+  }
 }
 
 int logits_check(Ctx *ctx, const char *what, const Buffer *xb, float scale) {
