@@ -152,10 +152,12 @@ __global__ void __launch_bounds__(THR, THR == 512 ? 4 : 1) logprobs_kernel(Logpr
   using C = Chunk16<T>;
   constexpr int E = C::E, NW = THR / 64;
   constexpr int STEP = NL < 4 ? NL : NL > 16 ? 2 : 4;  // chunks under one maximum
-  // The chunks and their maxima are kept in registers until the bound is
-  // known; more of them would spill: then the maxima wait in LDS and a chunk
-  // that reaches the bound is read again.
-  constexpr bool KEEP = NL <= 12 || NL * E < 96;
+  // Few chunks and their maxima are kept in registers until the bound is
+  // known; of more the maxima wait in LDS and a chunk that reaches the bound is
+  // read again, which leaves registers for more blocks a CU (4096 x 32000 BF16,
+  // top 5: 62.5 us, 70.7 with 8 chunks kept; 8192 x 8192 F32: 62.0, and
+  // 58.8 with its 4 kept).
+  constexpr bool KEEP = NL <= 4;
   __shared__ float red[NW][3];
   __shared__ float groups[64];
   __shared__ int ranks[NW][64];
