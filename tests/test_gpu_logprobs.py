@@ -140,6 +140,21 @@ def test_ties(eng, cols, elem):
 
 
 @pytest.mark.parametrize("elem", [F32, BF16])
+@pytest.mark.parametrize("cols", [4001, 9000, 33001, 49152, 98304])
+def test_as_many_equal_columns_as_there_is_room_for(eng, cols, elem):
+    """Around 1024 columns of the largest value, spread, at the front and at
+    the end, and a few above them."""
+    rng = np.random.default_rng(cols)
+    x = rng.standard_normal((15, cols)) - 8
+    for r, n in enumerate((1022, 1023, 1024, 1025, 1056)):
+        x[r, rng.permutation(cols)[:n]] = 2
+        x[5 + r, :n] = 2
+        x[10 + r, cols - n:] = 2
+        x[10 + r, rng.permutation(cols)[:3]] = 3
+    check(eng, x, elem, 1.0, 32)
+
+
+@pytest.mark.parametrize("elem", [F32, BF16])
 @pytest.mark.parametrize("cols", [100, 3001, 50000, 120000])
 def test_masked_logits(eng, cols, elem):
     """-inf in all places but some, and values near the type's lowest."""
