@@ -286,6 +286,32 @@ def test_backward(eng, rows, cols, elem, out):
     eng.sync()
 
 
+def test_more_rows_than_one_launch_holds(eng):
+    """A block a row is 2^24 - 1 blocks of 256 threads at most: the gradient
+    takes the rows in two launches, the forward refuses them."""
+    rows = 2**24 + 70
+    rng = np.random.default_rng(2)
+    x = rng.standard_normal((rows, 2)).astype(np.float32)
+    t = rng.integers(0, 2, rows).astype(np.int32)
+    g = rng.standard_normal(rows).astype(np.float32)
+    lse = np.logaddexp(x[:, 0], x[:, 1]).astype(np.float32)
+    xid, tid = eng.upload(x), eng.upload_i32(t.reshape(-1, 1))
+    lid, gid = eng.upload(lse.reshape(-1, 1)), eng.upload(g.reshape(-1, 1))
+    out = eng.token_logprobs_backward(xid, tid, lid, 0, gid, 0)
+    got = eng.download(out)
+    for at in (slice(0, 1000), slice(2**23 - 500, 2**23 + 500), slice(rows - 1000, rows)):
+        want, tol = grad64(x[at], 1.0, t[at], lse[at].astype(np.float64), np.zeros(len(t[at])), g[at], 0 * g[at])
+        assert np.all(np.abs(got[at] - want) <= tol)
+    before = eng.report()["live_buffers"]
+    with pytest.raises(miburn.MiError) as e:
+        eng.token_logprobs(xid, tid)
+    assert e.value.kind == "UNSUPPORTED"
+    assert eng.report()["live_buffers"] == before
+    for i in (xid, tid, lid, gid, out):
+        eng.free(i)
+    eng.sync()
+
+
 def test_backward_against_differences(eng):
     """sum(g logp + h entropy), its slope along random directions by central
     differences in 64 bits."""
