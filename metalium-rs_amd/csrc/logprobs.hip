@@ -143,10 +143,10 @@ __device__ __forceinline__ void put_top(const LogprobArgs &a, int64_t at, uint64
 // order from the row's start; a row with a NaN or +inf, and one whose columns
 // above the bound are too many, is searched k times.
 //
-// Measured: 2001 x 49152 F32, top 5: 64 us, 6.1 TB/s (without alternatives 60);
-// 64 x 49152 BF16, top 20: 10.1 us, 4.8 of it the sums (a block a CU, bound by
+// Measured: 2001 x 49152 F32, top 5: 63 us, 6.2 TB/s (without alternatives 60);
+// 64 x 49152 BF16, top 20: 9.7 us, 4.8 of it the sums (a block a CU, bound by
 // their operations), the rest five dependent steps of 0.3 to 2 us; 1 x 49152
-// F32, top 5: 8.2 us.
+// F32, top 5: 8.3 us.
 template <typename T, int THR, int NL, bool TOP, bool NT>
 __global__ void __launch_bounds__(THR, THR == 512 ? 4 : 1) logprobs_kernel(LogprobArgs a) {
   using C = Chunk16<T>;
@@ -584,8 +584,8 @@ __device__ __forceinline__ void store_grads(uint16_t *p, const float (&v)[E]) {
 
 // dx_j = scale (g ([j = target] - p_j) - h p_j (z_j - lse + H)), a chunk of E
 // elements a thread, from a boundary of both sides at or before the row: one
-// read and one write of each byte, bound by HBM.  2048 x 8192 F32 (134 MB): 23
-// us, 5.8 TB/s; 1001 x 40001 BF16 (160 MB): 29.6 us, 5.4 TB/s; a large copy
+// read and one write of each byte, bound by HBM.  2048 x 8192 F32 (134 MB): 21.7
+// us, 6.2 TB/s; 1001 x 40001 BF16 (160 MB): 30.5 us, 5.2 TB/s; a large copy
 // reaches 5.0.
 template <typename T, typename TO, bool NT>
 __global__ void __launch_bounds__(256) logprobs_backward_kernel(LogprobGradArgs a) {

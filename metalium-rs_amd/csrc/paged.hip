@@ -225,23 +225,6 @@ typedef float pa_f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int PA_WAVES = 4;
 constexpr int PA_HEADS = 16;       // query heads a block: the matrix cores' tile
-constexpr int64_t PA_BLOCKS = 512;   // blocks that run at once: two a CU
-constexpr int64_t PA_CHUNKS = 2048;  // chunks of one sequence at most: the join's weights in LDS
-// Chunk lengths are multiples of it.  80 sequences of up to 4074 (12 heads on
-// 1 of 128, F32): 37.9 us at 64, 41.7 at 128, 49.3 at 256; 180 of up to 500 (40 on 8 of
-// 128, BF16) 65.1, 60.0 and 59.9.
-constexpr int PA_UNIT = 128;
-// Positions up to which no sequence is cut, twice as many where the sequences
-// alone are a quarter of a round of blocks: no join, and no ends of chunks that do
-// not fit the blocks.  Heads 32 on 8 of 128, BF16: 64 sequences of 500 24.1
-// us whole, 34.1 cut; 8 of 256 6.6 and 9.3; 1 of 1000 12.8 and 9.4, 8 of 1000 14.3
-// and 12.4, 16 of 1000 15.0 and 18.8, 64 of 1000 44.1 and 51.5; 64 of up to 2000
-// 58.2 and 51.6.
-constexpr int64_t PA_WHOLE = 512;
-// Sequences up to which a wavefront forms the cut itself (with a launch before
-// it, 100 of up to 250, 9 heads on 3 of 64: 7.4 us, 10.7; 250 of up to 1000 26.1,
-// 28.6; 200 of up to 1000, 32 on 8 of 128, 91.1, 90.2).
-constexpr int64_t PA_SELF = 256;
 
 // Positions a wavefront takes a step: 8 KiB of keys at most.  80 sequences of
 // up to 4074, F32 keys of 128: 41.7 us at 16, 53.8 at 32; 32 of up to 2000, BF16
@@ -893,29 +876,16 @@ void attend_types(Ctx *ctx, const AttendArgs &a, unsigned grid, bool q16, bool k
 
 template <int D>
 int attend_launch(Ctx *ctx, AttendArgs a, bool q16, bool kv16) {
-  const int64_t parts = static_cast<int64_t>(a.kv_heads) * a.tiles, cap = a.per * a.page;
-  // Chunks for as many rounds of blocks as hold one a sequence twice: a cut
-  // leaves half a chunk a sequence more than the target on average.
-  // Where the sequences alone are many rounds only the longest are cut (700 of
-  // up to 300, 32 heads on 8 of 128: 175 us, 248 without this rule).
-  const int64_t round = PA_BLOCKS / parts > 1 ? PA_BLOCKS / parts : 1;
-  const int64_t rounds = (2 * a.seqs + round - 1) / round;
-  int64_t target = rounds * round - a.seqs / 2;
-  if (rounds > 8) target = a.seqs / 2 > 6 * round ? a.seqs / 2 : 6 * round;
-  const bool cut = cap > (a.seqs * parts >= PA_BLOCKS / 4 ? 2 : 1) * PA_WHOLE;
-  a.least = static_cast<int32_t>(cut ? (cap + PA_CHUNKS - 1) / PA_CHUNKS : cap);
-  // A sequence makes one chunk and at most one more a unit; all of them
-  // together at most the target's beside one each.
-  const int64_t most = cut ? (cap + PA_UNIT - 1) / PA_UNIT : 1;
-  int64_t chunks = target + a.seqs + 1;
-  if (most < chunks / a.seqs) chunks = most * a.seqs;
-  if (!cut) chunks = a.seqs;
+  const int64_t parts = static_cast<int64_t>(a.kv_heads) * a.tiles;
+  const PagedCut shape = paged_cut(a.seqs, a.per * a.page, parts);
+  const int64_t chunks = shape.chunks;
+  const bool cut = shape.cut, planned = a.seqs > PA_SELF;
+  a.least = static_cast<int32_t>(shape.least);
+  a.per_chunk = 1.0 / static_cast<double>(shape.target);
   a.chunks = chunks;
-  a.per_chunk = 1.0 / static_cast<double>(target);
-  a.slots = cut ? 2 * target + 2 : 0;
+  a.slots = shape.slots;
   if (chunks * parts > kGridThreads / 256 || a.seqs * a.heads > kGridThreads / 256)
     return fail(ctx, MI_E_UNSUPPORTED, "paged_attention: grid too large");
-  const bool planned = a.seqs > PA_SELF;
   const size_t cuts = cut ? (static_cast<size_t>(a.seqs) * sizeof(int2) + 255) / 256 * 256 : 0,
                plan = planned ? (static_cast<size_t>(chunks) * sizeof(int4) + 255) / 256 * 256 : 0,
                part = static_cast<size_t>(a.slots * parts * pa_stride(a.live, D)) * sizeof(float);

@@ -81,4 +81,58 @@ MI_HD int32_t chunk_len(int32_t len, int32_t n, int32_t unit) {
   return static_cast<int32_t>((units + n - 1) / n) * unit;
 }
 
+constexpr int64_t PA_BLOCKS = 512;   // blocks that run at once: two a CU
+constexpr int64_t PA_CHUNKS = 2048;  // chunks of one sequence at most: the join's weights in LDS
+// Chunk lengths are multiples of it.  80 sequences of up to 4074 (12 heads on
+// 1 of 128, F32): 37.9 us at 64, 41.7 at 128, 49.3 at 256; 180 of up to 500 (40 on 8 of
+// 128, BF16) 65.1, 60.0 and 59.9.
+constexpr int PA_UNIT = 128;
+// Positions up to which no sequence is cut, twice as many where the sequences
+// alone are a quarter of a round of blocks: no join, and no ends of chunks that do
+// not fit the blocks.  Heads 32 on 8 of 128, BF16: 64 sequences of 500 24.1
+// us whole, 34.1 cut; 8 of 256 6.6 and 9.3; 1 of 1000 12.8 and 9.4, 8 of 1000 14.3
+// and 12.4, 16 of 1000 15.0 and 18.8, 64 of 1000 44.1 and 51.5; 64 of up to 2000
+// 58.2 and 51.6.
+constexpr int64_t PA_WHOLE = 512;
+// Sequences up to which a wavefront forms the cut itself (with a launch before
+// it, 100 of up to 250, 9 heads on 3 of 64: 7.4 us, 10.7; 250 of up to 1000 26.1,
+// 28.6; 200 of up to 1000, 32 on 8 of 128, 91.1, 90.2).
+constexpr int64_t PA_SELF = 256;
+
+// The launch's shape for sequences of up to cap positions, `parts` blocks a
+// chunk.
+struct PagedCut {
+  bool cut;        // at all
+  int64_t target;  // chunks the lengths are cut for
+  int64_t least;   // positions a chunk at least
+  int64_t chunks;  // of all sequences at most
+  int64_t slots;   // of cut sequences at most
+};
+inline PagedCut paged_cut(int64_t seqs, int64_t cap, int64_t parts) {
+  PagedCut r;
+  // Chunks for as many rounds of blocks as hold one a sequence twice: a cut
+  // leaves half a chunk a sequence more than the target on average.
+  // Where the sequences alone are many rounds only the longest are cut (700 of
+  // up to 300, 32 heads on 8 of 128: 175 us, 248 without this rule).
+  const int64_t round = PA_BLOCKS / parts > 1 ? PA_BLOCKS / parts : 1;
+  const int64_t rounds = (2 * seqs + round - 1) / round;
+  r.target = rounds * round - seqs / 2;
+  if (rounds > 8) r.target = seqs / 2 > 6 * round ? seqs / 2 : 6 * round;
+  r.cut = cap > (seqs * parts >= PA_BLOCKS / 4 ? 2 : 1) * PA_WHOLE;
+  if (!r.cut) {
+    r.least = cap;
+    r.chunks = seqs;
+    r.slots = 0;
+    return r;
+  }
+  r.least = (cap + PA_CHUNKS - 1) / PA_CHUNKS;
+  // A sequence makes one chunk and at most one more a unit; all of them
+  // together at most the target's beside one each.
+  const int64_t most = (cap + PA_UNIT - 1) / PA_UNIT;
+  r.chunks = r.target + seqs + 1;
+  if (most < r.chunks / seqs) r.chunks = most * seqs;
+  r.slots = 2 * r.target + 2;
+  return r;
+}
+
 }  // namespace mi

@@ -17,5 +17,15 @@ int64_t limit_of(int64_t sum, int64_t target, int64_t least, int64_t unit) {
 }
 int32_t count_of(int32_t len, int64_t limit) { return mi::chunk_count(len, limit); }
 int32_t chunk_len_of(int32_t len, int32_t n, int32_t unit) { return mi::chunk_len(len, n, unit); }
+int cut_of(int64_t seqs, int64_t cap, int64_t parts, int64_t *shape) {
+  const mi::PagedCut c = mi::paged_cut(seqs, cap, parts);
+  shape[0] = c.target;
+  shape[1] = c.least;
+  shape[2] = c.chunks;
+  shape[3] = c.slots;
+  shape[4] = mi::PA_CHUNKS;
+  shape[5] = mi::PA_UNIT;
+  return c.cut;
+}
 int64_t len_of(int64_t len, int64_t cap) { return mi::paged_len(len, cap); }
 }

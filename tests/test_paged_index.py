@@ -30,6 +30,7 @@ def lib(tmp_path_factory):
     L.limit_of.argtypes, L.limit_of.restype = [I64] * 4, I64
     L.count_of.argtypes = [I32, I64]
     L.chunk_len_of.argtypes = [I32] * 3
+    L.cut_of.argtypes = [I64] * 3 + [ctypes.POINTER(I64)]
     L.len_of.argtypes, L.len_of.restype = [I64] * 2, I64
     return L
 
@@ -115,3 +116,27 @@ def test_chunks_cover_each_sequence_within_bounds(lib, unit):
                 slots += c if c > 1 else 0
             assert chunks <= target + 1 + len(lens)
             assert slots <= 2 * target + 2
+
+
+@pytest.mark.parametrize("seqs", [1, 2, 7, 63, 64, 65, 256, 257, 1000, 5000])
+@pytest.mark.parametrize("parts", [1, 3, 8, 16, 600])
+def test_chunks_fit_the_launch(lib, seqs, parts):
+    """For any lengths up to the table's positions: no more chunks than blocks,
+    no more chunks of cut sequences than partials, of one sequence than its
+    join holds; none cut where no join is launched."""
+    rng = random.Random(seqs * 31 + parts)
+    shape = (ctypes.c_int64 * 6)()
+    for cap in (0, 1, 511, 512, 513, 1024, 1025, 4096, 100_001, 3_000_000, I32_MAX):
+        cut = lib.cut_of(seqs, cap, parts, shape)
+        target, least, room, slots, most, unit = shape
+        for kind in range(6):
+            lens = {0: lambda: cap, 1: lambda: 0, 2: lambda: rng.randint(0, cap), 3: lambda: min(cap, 513),
+                    4: lambda: min(cap, rng.choice((0, 1, unit, unit + 1, 1100))),
+                    5: lambda: cap if rng.random() < 2 / seqs else min(cap, 3)}[kind]
+            lens = [lens() for _ in range(seqs)]
+            limit = lib.limit_of(sum(lens), target, least, unit)
+            counts = [lib.count_of(n, limit) for n in lens]
+            assert sum(counts) <= room
+            assert max(counts) <= (min(most, max(slots, 1)) if cut else 1)
+            assert sum(c for c in counts if c > 1) <= slots
+            assert all(lib.chunk_len_of(n, c, unit) * c >= n for n, c in zip(lens, counts))
