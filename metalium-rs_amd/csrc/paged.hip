@@ -884,7 +884,7 @@ int attend_launch(Ctx *ctx, AttendArgs a, bool q16, bool kv16) {
   a.per_chunk = 1.0 / static_cast<double>(shape.target);
   a.chunks = chunks;
   a.slots = shape.slots;
-  if (chunks * parts > kGridThreads / 256 || a.seqs * a.heads > kGridThreads / 256)
+  if (chunks * parts > kGridThreads / 256 || (cut && a.seqs * a.heads > kGridThreads / 256))
     return fail(ctx, MI_E_UNSUPPORTED, "paged_attention: grid too large");
   const size_t cuts = cut ? (static_cast<size_t>(a.seqs) * sizeof(int2) + 255) / 256 * 256 : 0,
                plan = planned ? (static_cast<size_t>(chunks) * sizeof(int4) + 255) / 256 * 256 : 0,

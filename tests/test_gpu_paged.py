@@ -401,6 +401,22 @@ def test_attention_shared_pages_and_repeated_rows(eng):
     attend_check(eng, c.up(eng), 8)
 
 
+@pytest.mark.parametrize("ce", [F32, BF16])
+@pytest.mark.parametrize("prompts,heads,kv,d,page", [([300], 4, 2, 32, 16), ([700, 5, 460], 3, 1, 64, 48),
+                                                     ([1300], 2, 1, 16, 16)])
+def test_attention_of_whole_prompts(eng, prompts, heads, kv, d, page, ce):
+    """A prompt's positions as rows: its table row repeated, each position
+    with its own length."""
+    rng = np.random.default_rng(sum(prompts))
+    one = Cache(rng, prompts, kv, d, page, ce).poison()
+    table, lens = [], []
+    for s, n in enumerate(prompts):
+        table += [one.table[s]] * n
+        lens += range(1, n + 1)
+    one.table, one.lens = np.array(table, np.int32), lens
+    attend_check(eng, one.up(eng), heads)
+
+
 def test_attention_equals_contiguous_cache(eng):
     """One slot a sequence: mi_attention_rows_at's values within both
     kernels' tolerances."""
