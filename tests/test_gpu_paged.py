@@ -674,6 +674,40 @@ def test_trace_replays_at_any_lengths(eng):
     eng.release_trace(trace)
 
 
+@pytest.mark.parametrize("seqs,most", [(100, 700), (300, 700), (300, 300)])
+def test_trace_of_many_sequences_replays_at_any_lengths(eng, seqs, most):
+    """The attention of many sequences captured once: lengths that change
+    between replays, eager calls of another size in between."""
+    rng = np.random.default_rng(seqs + most)
+    c = Cache(rng, [most] * seqs, 1, 32, 16, BF16).up(eng)
+    few = Cache(rng, [3000, 40], 1, 32, 16, F32).poison().up(eng)
+    q, fq = (eng.upload(rng.standard_normal((n, 64))) for n in (seqs, 2))
+    lens = eng.upload_i32(np.zeros((seqs, 1)))
+    eng.begin_trace()
+    out = eng.paged_attention(q, c.kid, c.vid, c.tid, lens, 2, 1, 16, 0.25)
+    trace = eng.end_trace()
+    other = eng.download(eng.paged_attention(fq, few.kid, few.vid, few.tid, few.lid, 2, 1, 16, 0.25))
+    for turn in range(5):
+        ls = rng.integers(0, most + 1, (seqs, 1)).astype(np.int32)
+        if turn == 2:
+            ls[:] = 0
+        if turn == 3:
+            ls[:] = 1
+            ls[seqs // 2] = most
+        got, = eng.run_trace(trace, {lens: ls}, [out])
+        o = eng.paged_attention(fq, few.kid, few.vid, few.tid, few.lid, 2, 1, 16, 0.25)
+        assert np.array_equal(bits(eng.download(o)), bits(other))
+        c.lens = ls[:, 0].tolist()
+        want, tol = attend64(c, eng.download(q), 2, 0.25)
+        assert np.all(np.abs(got - want) <= tol), turn
+        eager = eng.paged_attention(q, c.kid, c.vid, c.tid, lens, 2, 1, 16, 0.25)
+        assert np.array_equal(bits(got), bits(eng.download(eager))), turn
+        eng.free(o)
+        eng.free(eager)
+        eng.sync()
+    eng.release_trace(trace)
+
+
 def test_two_traces_and_eager_calls_share_the_scratch(eng):
     """Two captured calls of unequal sizes and eager ones between them."""
     rng = np.random.default_rng(19)
